@@ -22,7 +22,7 @@ from typing import List
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
-HIP_SOURCES = ["gemm.hip", "loss.hip", "optim.hip", "replay.hip", "nstep.hip", "fused.hip", "fused32.hip", "rollout.hip", "planar_env.hip", "analytic_env.hip", "ant_env.hip"]
+HIP_SOURCES = ["gemm.hip", "loss.hip", "optim.hip", "replay.hip", "nstep.hip", "fused.hip", "fused32.hip", "rollout.hip", "int8.hip", "planar_env.hip", "analytic_env.hip", "ant_env.hip"]
 HOST_SOURCES = ["host_runtime.cpp", "planar_host.cpp"]
 HIP_LIB = os.path.join(CSRC, "libd4pg_hip.so")
 HOST_LIB = os.path.join(CSRC, "libd4pg_host.so")
@@ -112,6 +112,11 @@ FUSED_PARTS = {"fused.hip": (-1, 13, 4, 8, 0), "fused32.hip": (-1, 13, 4, 8, 2, 
 #: to the host simulator step by step at whatever level is built).
 OPT_LEVEL: dict = {"ant_env.hip": "-O1"}
 
+#: further flags per source.  int8.hip: no packed fp32 arithmetic, which hipcc makes from ordinary float code by itself (the
+#: host pass does not know the feature and warns; that is harmless).  The learner's kernels keep the code generation their
+#: results were pinned with: without it a few hidden values land on the other side of a ReLU
+EXTRA_FLAGS: dict = {"int8.hip": ("-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops")}
+
 
 def _hip_units(stamps: bool):
     """(source, part, object path, command) of every translation unit of the HIP library."""
@@ -128,7 +133,7 @@ def _hip_units(stamps: bool):
             # --offload-compress: the gfx950 code objects are stored compressed in the fat binary (the HIP runtime inflates
             # them at load): the library shrinks from 15.9 to about 4 MB, which every copy of the tree to a GPU box pays for
             cmd = [hipcc, OPT_LEVEL.get(name, "-O3"), f"--offload-arch={ARCH}", "--offload-compress", "-fPIC", "-std=c++17",
-                   "-c", s, "-o", o]
+                   *EXTRA_FLAGS.get(name, ()), "-c", s, "-o", o]
             if part is not None:
                 cmd.insert(1, f"-DD4PG_KSH_PART={part}")
             if stamps:

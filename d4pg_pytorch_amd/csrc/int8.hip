@@ -1,0 +1,553 @@
+// 8-bit serving operators for gfx950: rows to codes and back, RMS norm with 8-bit output, int8 product.
+//
+// A quantised row is 127-level symmetric: a = max_k |y_k|, scale s = a / 127, code q_k = rint(y_k * 127 / a), so that
+// y_k ~ q_k * s.  All codes of a row share s; the product of two quantised matrices is then
+//
+//     y[m, n] = act( (sum_k q[m, k] p[n, k]) * s[m] * t[n] + b[n] )
+//
+// with the sum exact in 32-bit integers (K < 2^31 / 128^2 = 131072) and everything after it in fp32.
+//
+// Conventions
+//  * Code matrices are row-major with 16-byte aligned rows: the row stride is a multiple of 16 and at least K rounded up
+//    to 16, and every byte up to there is readable.  The bytes beyond K may hold anything: the product clears them in
+//    the ACTIVATION operand (0 * anything = 0 in integers, so one operand suffices).
+//  * A row that holds a NaN or an infinity gets scale NaN and codes 0: whatever reads it gets NaN, never a number.
+//  * A row of zeros gets scale 0 and codes 0.
+#include "common.h"
+
+enum { F_FP32 = 0, F_BF16 = 1, F_FP16 = 2, F_NONE = -1 };
+enum { ACT_NONE = 0, ACT_RELU = 1, ACT_TANH = 2 };
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+
+// ---------------------------------------------------------------------------------------------------------------
+// floating rows -> codes
+// ---------------------------------------------------------------------------------------------------------------
+struct QuantRowsArgs {
+    const void* x;         // [M, K] rows of ld_x elements
+    const void* residual;  // [M, K] added to x, or null                       (norm only)
+    const void* weight;    // [K] factor after the norm, or null               (norm only)
+    void* h;               // [M, K] x + residual in x's type, or null         (norm only)
+    signed char* q;        // [M, ld_q] codes, zero from K to ld_q
+    float* scale;          // [M]
+    long long M, K;
+    long long ld_x, ld_r, ld_h, ld_q;   // elements (bytes for ld_q, a multiple of 16)
+    int dtype, wdtype;     // F_*: of x, residual and h; of weight
+    int norm;              // 0: quantise x; 1: RMS norm first
+    float eps;
+};
+
+// Eight neighbouring elements of a row.  Only the element's own alignment is assumed: gfx950 takes 16-byte loads and
+// stores at any address, so rows of odd length need no path of their own (the last K % 8 elements aside).
+template <typename T>
+struct Raw8 {
+    T e[8];
+};
+template <typename T>
+__device__ __forceinline__ Raw8<T> load8(const T* p) {
+    Raw8<T> r;
+    __builtin_memcpy(&r, p, sizeof(r));
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+    Raw8<T> r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.e[i] = (T)v[i];
+    __builtin_memcpy(p, &r, sizeof(r));
+}
+
+__device__ __forceinline__ unsigned wave_umax(unsigned v) {
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xb1, 0xf, 0xf, false));
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4e, 0xf, 0xf, false));
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false));
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false));
+    const unsigned a = __builtin_amdgcn_readlane((int)v, 0), b = __builtin_amdgcn_readlane((int)v, 16);
+    const unsigned c = __builtin_amdgcn_readlane((int)v, 32), d = __builtin_amdgcn_readlane((int)v, 48);
+    return max(max(a, b), max(c, d));
+}
+
+// Sum / maximum over the G threads that share a row.  G = 64: one wave, no LDS.  `red` holds 32 words; two of them
+// alternate between calls so that one barrier a call is enough.
+template <int G>
+__device__ __forceinline__ float group_sum(float v, unsigned* red) {
+    v = wave_sum(v);
+    if constexpr (G == 64) return v;
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = __builtin_bit_cast(unsigned, v);
+    __syncthreads();
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < G / 64; ++w) s += __builtin_bit_cast(float, red[w]);
+    return s;
+}
+template <int G>
+__device__ __forceinline__ unsigned group_umax(unsigned v, unsigned* red) {
+    v = wave_umax(v);
+    if constexpr (G == 64) return v;
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    unsigned s = 0;
+#pragma unroll
+    for (int w = 0; w < G / 64; ++w) s = max(s, red[w]);
+    return s;
+}
+
+__device__ __forceinline__ unsigned abs_bits(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
+
+// What turns a row's values into codes.  |y| as an unsigned integer orders like the value, with infinity and NaN above
+// every finite number, so one integer maximum finds the largest magnitude and whether the row is finite.
+struct RowCode {
+    float pre, inv, scale;
+    unsigned keep;         // all ones, or 0 for a row that is not finite
+};
+__device__ __forceinline__ RowCode row_code(unsigned top_bits) {
+    const float top = __builtin_bit_cast(float, top_bits);
+    RowCode c;
+    const bool finite = top_bits < 0x7f800000u;
+    // 127 / top overflows for the smallest rows: those are lifted by 2^64 first (exact)
+    c.pre = top < 0x1p-62f ? 0x1p64f : 1.f;
+    c.inv = top > 0.f && finite ? 127.f / (top * c.pre) : 0.f;
+    c.scale = finite ? top / 127.f : __builtin_nanf("");
+    c.keep = finite ? ~0u : 0u;
+    return c;
+}
+// rint(y * 127 / a) as a byte: adding 1.5 * 2^23 leaves the rounded integer, halves to even, in the low bits.  The product is
+// rounded on its own: where y / a is exactly halfway between two codes that restores the half which 127 / a had lost.
+__device__ __forceinline__ unsigned code_bits(float y, const RowCode& c) {
+#pragma clang fp contract(off)
+    const float v = y * c.pre * c.inv;
+    return __builtin_bit_cast(unsigned, v + 12582912.f);
+}
+__device__ __forceinline__ unsigned pack4(unsigned a, unsigned b, unsigned c, unsigned d) {
+    const unsigned lo = __builtin_amdgcn_perm(b, a, 0x0c0c0400u), hi = __builtin_amdgcn_perm(d, c, 0x04000c0cu);
+    return lo | hi;
+}
+__device__ __forceinline__ void store_codes8(signed char* p, const float (&y)[8], const RowCode& c) {
+    uint2 w;
+    w.x = pack4(code_bits(y[0], c), code_bits(y[1], c), code_bits(y[2], c), code_bits(y[3], c)) & c.keep;
+    w.y = pack4(code_bits(y[4], c), code_bits(y[5], c), code_bits(y[6], c), code_bits(y[7], c)) & c.keep;
+    *reinterpret_cast<uint2*>(p) = w;
+}
+
+// The factor of the norm.  The plain sum of squares overflows above ~1.8e19 and loses everything below ~1e-20; a row
+// like that (known from the sum itself, so that ordinary rows pay nothing) is scaled by a power of two first.
+struct NormFactor {
+    float pre, rs;         // y = (h * pre) * rs * weight
+};
+__device__ __forceinline__ bool norm_is_plain(float ss, float K, float eps) {
+    const float ms = ss / K + eps;
+    return ms >= 0x1p-80f && ss < __builtin_inff();
+}
+__device__ __forceinline__ float norm_lift(unsigned top_bits, float eps) {
+    int e = (int)(top_bits >> 23) - 126;
+    if (top_bits < 0x00800000u) e = -126;
+    if (eps > 0.f && e < -60) e = -60;         // below that the added eps decides, and must stay finite
+    e = e < -120 ? -120 : (e > 126 ? 126 : e);
+    return __builtin_ldexpf(1.f, -e);
+}
+
+template <typename T>
+__device__ __forceinline__ float load1(const void* p, long long i) {
+    return (float)reinterpret_cast<const T*>(p)[i];
+}
+__device__ __forceinline__ float weight1(const QuantRowsArgs& a, long long k) {
+    if (a.wdtype == F_FP32) return load1<float>(a.weight, k);
+    if (a.wdtype == F_BF16) return load1<__bf16>(a.weight, k);
+    if (a.wdtype == F_FP16) return load1<_Float16>(a.weight, k);
+    return 1.f;
+}
+template <typename W>
+__device__ __forceinline__ void scale8(float (&y)[8], const void* weight, long long k) {
+    const Raw8<W> w = load8(reinterpret_cast<const W*>(weight) + k);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] *= (float)w.e[i];
+}
+
+// A row stays in the registers of its G threads from the load to the codes: one read, one write, whatever is computed
+// between.  Thread t holds the 8-element chunks t, t + G, ... (V of them).
+template <typename T, int G, int V, bool NORM>
+__global__ __launch_bounds__(G < 256 ? 256 : G) void quant_rows_kernel(const QuantRowsArgs a) {
+    constexpr int BLOCK = G < 256 ? 256 : G;
+    __shared__ unsigned red[4][G > 64 ? G / 64 : 1];
+    const long long row = (long long)blockIdx.x * (BLOCK / G) + threadIdx.x / G;
+    if (row >= a.M) return;                      // whole waves (G = 64) only: no barrier is skipped
+    const int t = threadIdx.x % G;
+    const int K = (int)a.K, full = K >> 3, rem = K & 7, chunks = (int)(a.ld_q >> 3);
+    const T* const x = reinterpret_cast<const T*>(a.x) + row * a.ld_x;
+    const T* const r = reinterpret_cast<const T*>(a.residual) + row * a.ld_r;
+    const bool add = NORM && a.residual != nullptr;
+
+    float y[V][8];
+    {
+        // every thread loads from an address inside the row and drops what lies beyond it, so that all loads are in
+        // flight at once
+        Raw8<T> rx[V], rr[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = min(t + j * G, full - 1);
+            if (full > 0) rx[j] = load8(x + 8 * c);
+        }
+        if (add) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const int c = min(t + j * G, full - 1);
+                if (full > 0) rr[j] = load8(r + 8 * c);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = t + j * G;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float v = (float)rx[j].e[i];
+                if (add) v += (float)rr[j].e[i];
+                y[j][i] = c < full ? v : 0.f;
+            }
+            if (c == full && rem) {              // the last elements of a row whose length is no multiple of 8
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i < rem) y[j][i] = (float)x[8 * c + i] + (add ? (float)r[8 * c + i] : 0.f);
+            }
+        }
+    }
+    if (NORM) {
+        if (a.h != nullptr) {
+            T* const h = reinterpret_cast<T*>(a.h) + row * a.ld_h;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const int c = t + j * G;
+                if (c < full) store8(h + 8 * c, y[j]);
+                if (c == full && rem) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (i < rem) h[8 * c + i] = (T)y[j][i];
+                }
+            }
+        }
+        float ss = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss += y[j][i] * y[j][i];
+        ss = group_sum<G>(ss, red[0]);
+        float pre = 1.f, eps = a.eps;
+        if (!norm_is_plain(ss, (float)K, eps)) { // the same for the whole row
+            unsigned top = 0;
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = max(top, abs_bits(y[j][i]));
+            top = group_umax<G>(top, red[1]);
+            pre = norm_lift(top, eps);
+            ss = 0.f;
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) ss += (y[j][i] * pre) * (y[j][i] * pre);
+            ss = group_sum<G>(ss, red[2]);
+            eps = eps * pre * pre;
+            if (top >= 0x7f800000u) ss = __builtin_nanf("");
+            if (top == 0u && a.eps == 0.f) eps = 1.f;      // a row of zeros stays one
+        }
+        const float rs = 1.f / sqrtf(ss / (float)K + eps);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = t + j * G;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[j][i] = (y[j][i] * pre) * rs;
+            if (a.wdtype != F_NONE) {
+                if (c < full) {
+                    if (a.wdtype == F_FP32) scale8<float>(y[j], a.weight, 8 * c);
+                    else if (a.wdtype == F_BF16) scale8<__bf16>(y[j], a.weight, 8 * c);
+                    else scale8<_Float16>(y[j], a.weight, 8 * c);
+                } else if (c == full && rem) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (i < rem) y[j][i] *= weight1(a, 8 * c + i);
+                }
+            }
+        }
+    }
+    unsigned top = 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, abs_bits(y[j][i]));
+    const RowCode code = row_code(group_umax<G>(top, red[3]));
+    signed char* const q = a.q + row * a.ld_q;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int c = t + j * G;
+        if (c < chunks) store_codes8(q + 8 * c, y[j], code);
+    }
+    if (t == 0) a.scale[row] = code.scale;
+}
+
+// Rows too long for the registers of 1024 threads: the row is read again for each of the three steps.
+template <typename T, bool NORM>
+__global__ __launch_bounds__(1024) void quant_long_rows_kernel(const QuantRowsArgs a) {
+    constexpr int G = 1024;
+    __shared__ unsigned red[4][G / 64];
+    const long long row = blockIdx.x;
+    const T* const x = reinterpret_cast<const T*>(a.x) + row * a.ld_x;
+    const T* const r = reinterpret_cast<const T*>(a.residual) + row * a.ld_r;
+    T* const h = reinterpret_cast<T*>(a.h) + row * a.ld_h;
+    const bool add = NORM && a.residual != nullptr;
+    const long long K = a.K;
+    auto value = [&](long long k) { return (float)x[k] + (add ? (float)r[k] : 0.f); };
+    float pre = 1.f, rs = 1.f;
+    if (NORM) {
+        float ss = 0.f;
+        for (long long k = threadIdx.x; k < K; k += G) {
+            const float v = value(k);
+            ss += v * v;
+            if (a.h != nullptr) h[k] = (T)v;
+        }
+        ss = group_sum<G>(ss, red[0]);
+        float eps = a.eps;
+        if (!norm_is_plain(ss, (float)K, eps)) {
+            unsigned top = 0;
+            for (long long k = threadIdx.x; k < K; k += G) top = max(top, abs_bits(value(k)));
+            top = group_umax<G>(top, red[1]);
+            pre = norm_lift(top, eps);
+            ss = 0.f;
+            for (long long k = threadIdx.x; k < K; k += G) {
+                const float v = value(k) * pre;
+                ss += v * v;
+            }
+            ss = group_sum<G>(ss, red[2]);
+            eps = eps * pre * pre;
+            if (top >= 0x7f800000u) ss = __builtin_nanf("");
+            if (top == 0u && a.eps == 0.f) eps = 1.f;
+        }
+        rs = 1.f / sqrtf(ss / (float)K + eps);
+    }
+    auto out = [&](long long k) { return NORM ? (value(k) * pre) * rs * weight1(a, k) : value(k); };
+    unsigned top = 0;
+    for (long long k = threadIdx.x; k < K; k += G) top = max(top, abs_bits(out(k)));
+    const RowCode code = row_code(group_umax<G>(top, red[3]));
+    signed char* const q = a.q + row * a.ld_q;
+    for (long long k = threadIdx.x; k < a.ld_q; k += G)
+        q[k] = k < K ? (signed char)(code_bits(out(k), code) & code.keep) : 0;
+    if (threadIdx.x == 0) a.scale[row] = code.scale;
+}
+
+template <typename T, int G, int V>
+static void launch_rows(const QuantRowsArgs& a, hipStream_t stream) {
+    constexpr int BLOCK = G < 256 ? 256 : G, RPB = BLOCK / G;
+    const dim3 grid((unsigned)((a.M + RPB - 1) / RPB)), block(BLOCK);
+    if (a.norm) hipLaunchKernelGGL((quant_rows_kernel<T, G, V, true>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((quant_rows_kernel<T, G, V, false>), grid, block, 0, stream, a);
+}
+template <typename T>
+static void launch_rows_of(const QuantRowsArgs& a, hipStream_t stream) {
+    // chunks of 8 a row needs: as few threads as hold it in at most 4 (8 from 8192 columns) chunks each
+    const long long c = a.ld_q >> 3;
+    if (c <= 64) launch_rows<T, 64, 1>(a, stream);
+    else if (c <= 128) launch_rows<T, 64, 2>(a, stream);
+    else if (c <= 256) launch_rows<T, 64, 4>(a, stream);
+    else if (c <= 512) launch_rows<T, 256, 2>(a, stream);
+    else if (c <= 1024) launch_rows<T, 256, 4>(a, stream);
+    else if (c <= 2048) launch_rows<T, 256, 8>(a, stream);
+    else if (c <= 4096) launch_rows<T, 1024, 4>(a, stream);
+    else {
+        const dim3 grid((unsigned)a.M), block(1024);
+        if (a.norm) hipLaunchKernelGGL((quant_long_rows_kernel<T, true>), grid, block, 0, stream, a);
+        else hipLaunchKernelGGL((quant_long_rows_kernel<T, false>), grid, block, 0, stream, a);
+    }
+}
+
+D4PG_API int d4pg_quant_rows(const QuantRowsArgs* a, hipStream_t stream) {
+    if (a->M < 1 || a->M > 0x7fffffffll || a->K < 1 || a->K > 0x7fffffffll) return -1;
+    if (a->x == nullptr || a->q == nullptr || a->scale == nullptr) return -2;
+    if ((a->ld_q & 15) || a->ld_q < a->K || a->ld_q >= a->K + 16 || ((uintptr_t)a->q & 15)) return -3;
+    if (a->wdtype != F_NONE && (a->weight == nullptr || a->wdtype < 0 || a->wdtype > F_FP16)) return -4;
+    if (!a->norm && (a->residual != nullptr || a->weight != nullptr || a->h != nullptr)) return -5;
+    if (a->dtype == F_FP32) launch_rows_of<float>(*a, stream);
+    else if (a->dtype == F_BF16) launch_rows_of<__bf16>(*a, stream);
+    else if (a->dtype == F_FP16) launch_rows_of<_Float16>(*a, stream);
+    else return -6;
+    return (int)hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// codes -> floating rows
+// ---------------------------------------------------------------------------------------------------------------
+struct DequantRowsArgs {
+    const signed char* q;  // [M, K] rows of ld_q bytes
+    const float* scale;    // [M]
+    void* out;             // [M, K] contiguous
+    long long M, K, ld_q;
+    int dtype, tpr_log;    // threads a row = 2^tpr_log (set by the host entry)
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void dequant_rows_kernel(const DequantRowsArgs a) {
+    const int tpr = 1 << a.tpr_log;
+    const long long row = (long long)blockIdx.x * (256 >> a.tpr_log) + (threadIdx.x >> a.tpr_log);
+    if (row >= a.M) return;
+    const float s = a.scale[row];
+    const signed char* const q = a.q + row * a.ld_q;
+    T* const out = reinterpret_cast<T*>(a.out) + row * a.K;
+    for (long long k = 8ll * (threadIdx.x & (tpr - 1)); k < a.K; k += 8ll * tpr) {
+        if (k + 8 <= a.K) {
+            const Raw8<signed char> c = load8(q + k);
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = (float)c.e[i] * s;
+            store8(out + k, v);
+        } else {
+            for (long long i = k; i < a.K; ++i) out[i] = (T)((float)q[i] * s);
+        }
+    }
+}
+
+D4PG_API int d4pg_dequant_rows(DequantRowsArgs* a, hipStream_t stream) {
+    if (a->M < 1 || a->M > 0x7fffffffll || a->K < 1 || a->K > 0x7fffffffll) return -1;
+    if (a->q == nullptr || a->scale == nullptr || a->out == nullptr) return -2;
+    a->tpr_log = 0;
+    while (a->tpr_log < 8 && (8ll << a->tpr_log) < a->K) ++a->tpr_log;
+    const int rpb = 256 >> a->tpr_log;
+    const dim3 grid((unsigned)((a->M + rpb - 1) / rpb)), block(256);
+    if (a->dtype == F_FP32) hipLaunchKernelGGL(dequant_rows_kernel<float>, grid, block, 0, stream, *a);
+    else if (a->dtype == F_BF16) hipLaunchKernelGGL(dequant_rows_kernel<__bf16>, grid, block, 0, stream, *a);
+    else if (a->dtype == F_FP16) hipLaunchKernelGGL(dequant_rows_kernel<_Float16>, grid, block, 0, stream, *a);
+    else return -6;
+    return (int)hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// product of codes
+// ---------------------------------------------------------------------------------------------------------------
+struct LinearInt8Args {
+    const signed char* q;  // [M, K] activations' codes, rows of ld_q bytes
+    const float* scale;    // [M]
+    const signed char* w;  // [N, K] weights' codes, rows of ld_w bytes
+    const float* wscale;   // [N]
+    const float* bias;     // [N] or null
+    void* out;             // [M, N], rows of ld_out elements
+    long long ld_q, ld_w, ld_out;
+    int M, N, K;
+    int act, dtype, pad_;
+};
+
+__device__ __forceinline__ float act_of(float y, int act) {
+    if (act == ACT_RELU) return y < 0.f ? 0.f : y;        // keeps NaN
+    if (act == ACT_TANH) return tanhf(y);
+    return y;
+}
+// Four neighbouring columns n .. n + 3 of row m (those below N).  v: integer sums.
+template <typename T>
+__device__ __forceinline__ void store4(T* out, const float (&v)[4], int left) {
+    if (left >= 4) {
+        T r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = (T)v[i];
+        __builtin_memcpy(out, r, sizeof(r));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (i < left) out[i] = (T)v[i];
+    }
+}
+__device__ __forceinline__ void finish4(const LinearInt8Args& a, int m, int n, const i32x4 sum, float sm) {
+    if (m >= a.M || n >= a.N) return;
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int ni = min(n + i, a.N - 1);
+        v[i] = ((float)sum[i] * sm) * a.wscale[ni];
+        if (a.bias != nullptr) v[i] += a.bias[ni];
+        v[i] = act_of(v[i], a.act);
+    }
+    const long long o = (long long)m * a.ld_out + n;
+    if (a.dtype == F_FP32) store4(reinterpret_cast<float*>(a.out) + o, v, a.N - n);
+    else if (a.dtype == F_BF16) store4(reinterpret_cast<__bf16*>(a.out) + o, v, a.N - n);
+    else store4(reinterpret_cast<_Float16*>(a.out) + o, v, a.N - n);
+}
+
+// All ones in the bytes k .. k + 15 that lie below K.
+__device__ __forceinline__ i32x4 below(int k, int K) {
+    i32x4 m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int left = K - (k + 4 * i);
+        m[i] = left >= 4 ? -1 : (left <= 0 ? 0 : (int)((1u << (8 * left)) - 1u));
+    }
+    return m;
+}
+
+// Few rows or small layers: a workgroup makes 16 MT rows x 16 NT columns, its WAVES waves split K and meet in LDS.
+// Operands go from memory to the matrix instruction's registers directly (v_mfma_i32_16x16x64_i8: lane 16 g + c holds
+// 16 bytes of row c at k = 16 g); the weights are the A operand, so that a lane ends with four neighbouring columns.
+template <int MT, int NT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void linear_int8_rows_kernel(const LinearInt8Args a) {
+    __shared__ i32x4 part[WAVES][MT * NT][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 15, g = lane >> 4;
+    const int tiles_n = (a.N + 16 * NT - 1) / (16 * NT);
+    const int tm = blockIdx.x / tiles_n, tn = blockIdx.x - tm * tiles_n;
+    const signed char* xp[MT];
+    const signed char* wp[NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) xp[i] = a.q + (long long)min((tm * MT + i) * 16 + c, a.M - 1) * a.ld_q;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) wp[i] = a.w + (long long)min((tn * NT + i) * 16 + c, a.N - 1) * a.ld_w;
+    const int last = ((a.K - 1) >> 4) << 4;      // the last 16 bytes of a row that hold a code
+    i32x4 acc[MT][NT] = {};
+    // step s of the wave covers k = 64 (wave + s WAVES): neighbouring waves read neighbouring bytes
+    for (int k0 = 64 * wave; k0 < a.K; k0 += 64 * WAVES) {
+        const int k = k0 + 16 * g, kc = min(k, last);
+        i32x4 x[MT], w[NT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) w[i] = *reinterpret_cast<const i32x4*>(wp[i] + kc);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) x[i] = *reinterpret_cast<const i32x4*>(xp[i] + kc);
+        if (k0 + 64 > a.K) {
+            const i32x4 m = below(k, a.K);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) x[i] &= m;
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[j], x[i], acc[i][j], 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) part[wave][i * NT + j][lane] = acc[i][j];
+    __syncthreads();
+    for (int u = wave; u < MT * NT; u += WAVES) {
+        i32x4 sum = part[0][u][lane];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) sum += part[w][u][lane];
+        const int m = (tm * MT + u / NT) * 16 + c, n = (tn * NT + u % NT) * 16 + 4 * g;
+        finish4(a, m, n, sum, a.scale[min(m, a.M - 1)]);
+    }
+}
+
+template <int MT, int NT, int WAVES>
+static void launch_linear_rows(const LinearInt8Args& a, hipStream_t stream) {
+    const long long tiles = (long long)((a.M + 16 * MT - 1) / (16 * MT)) * ((a.N + 16 * NT - 1) / (16 * NT));
+    hipLaunchKernelGGL((linear_int8_rows_kernel<MT, NT, WAVES>), dim3((unsigned)tiles), dim3(64 * WAVES), 0, stream, a);
+}
+
+D4PG_API int d4pg_linear_int8(const LinearInt8Args* a, hipStream_t stream) {
+    if (a->M < 1 || a->N < 1 || a->K < 1 || a->K >= 131072) return -1;
+    if (a->q == nullptr || a->w == nullptr || a->scale == nullptr || a->wscale == nullptr || a->out == nullptr) return -2;
+    const long long kp = (a->K + 15) & ~15;
+    if (((a->M > 1 ? a->ld_q : 16) & 15) || ((a->N > 1 ? a->ld_w : 16) & 15)) return -3;
+    if ((a->M > 1 && a->ld_q < kp) || (a->N > 1 && a->ld_w < kp) || (a->M > 1 && a->ld_out < a->N)) return -4;
+    if (((uintptr_t)a->q | (uintptr_t)a->w) & 15) return -5;
+    if (a->dtype < F_FP32 || a->dtype > F_FP16 || a->act < ACT_NONE || a->act > ACT_TANH) return -6;
+    if ((long long)((a->M + 15) / 16) * ((a->N + 15) / 16) > 0x7fffffffll) return -7;
+    if (a->M <= 16) launch_linear_rows<1, 1, 4>(*a, stream);
+    else launch_linear_rows<2, 2, 4>(*a, stream);
+    return (int)hipGetLastError();
+}
+
+D4PG_SIZEOF(QuantRowsArgs)
+D4PG_SIZEOF(DequantRowsArgs)
+D4PG_SIZEOF(LinearInt8Args)

@@ -29,6 +29,8 @@ _lib: Optional[C.CDLL] = None
 # ---------------------------------------------------------------------------
 GEMM_NT, GEMM_NN, GEMM_TN = 0, 1, 2
 EPI_NONE, EPI_RELU, EPI_TANH, EPI_MUL_RELU_MASK, EPI_MUL_TANH_GRAD = 0, 1, 2, 3, 4
+F_NONE, F_FP32, F_BF16, F_FP16 = -1, 0, 1, 2           # floating types of csrc/int8.hip
+ACT_NONE, ACT_RELU, ACT_TANH = 0, 1, 2
 MAX_GROUP = 6
 MAXL = 6
 
@@ -371,6 +373,25 @@ class OuArgs(C.Structure):
                 ("low", C.c_float), ("high", C.c_float)]
 
 
+# ---- 8-bit serving operators (csrc/int8.hip) ----
+class QuantRowsArgs(C.Structure):
+    _fields_ = [("x", vp), ("residual", vp), ("weight", vp), ("h", vp), ("q", vp), ("scale", vp),
+                ("M", C.c_longlong), ("K", C.c_longlong),
+                ("ld_x", C.c_longlong), ("ld_r", C.c_longlong), ("ld_h", C.c_longlong), ("ld_q", C.c_longlong),
+                ("dtype", C.c_int), ("wdtype", C.c_int), ("norm", C.c_int), ("eps", C.c_float)]
+
+
+class DequantRowsArgs(C.Structure):
+    _fields_ = [("q", vp), ("scale", vp), ("out", vp), ("M", C.c_longlong), ("K", C.c_longlong), ("ld_q", C.c_longlong),
+                ("dtype", C.c_int), ("tpr_log", C.c_int)]
+
+
+class LinearInt8Args(C.Structure):
+    _fields_ = [("q", vp), ("scale", vp), ("w", vp), ("wscale", vp), ("bias", vp), ("out", vp),
+                ("ld_q", C.c_longlong), ("ld_w", C.c_longlong), ("ld_out", C.c_longlong),
+                ("M", C.c_int), ("N", C.c_int), ("K", C.c_int), ("act", C.c_int), ("dtype", C.c_int), ("pad_", C.c_int)]
+
+
 class DevStateMirror(C.Structure):
     """Host mirror of ``struct DevState`` (csrc/common.h) for init / read-back."""
     _fields_ = [("step_done", C.c_longlong), ("step_cur", C.c_longlong),
@@ -469,6 +490,9 @@ def lib() -> C.CDLL:
             ("d4pg_analytic_env_step", [C.POINTER(AnalyticEnvArgs), vp]),
             ("d4pg_ant_env_step", [C.POINTER(AntEnvArgs), C.POINTER(AntParams), vp]),
             ("d4pg_rollout_rows", [C.POINTER(RolloutRowsArgs), vp]),
+            ("d4pg_quant_rows", [C.POINTER(QuantRowsArgs), vp]),
+            ("d4pg_dequant_rows", [C.POINTER(DequantRowsArgs), vp]),
+            ("d4pg_linear_int8", [C.POINTER(LinearInt8Args), vp]),
             ("d4pg_ipc_alloc", [C.c_size_t, C.POINTER(vp), C.c_char_p]),
             ("d4pg_ipc_open", [C.c_char_p, C.POINTER(vp)]),
             ("d4pg_ipc_close", [vp]),

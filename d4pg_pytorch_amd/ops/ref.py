@@ -270,3 +270,47 @@ def mlp3(x, w1, b1, w2, b2, w3, b3, final: str = "none"):
     elif final == "softmax":
         y = torch.softmax(y, dim=1)
     return y
+
+
+# ---------------------------------------------------------------------------
+# 8-bit serving operators (codes of a row share one scale; rows of a matrix [M, K])
+# ---------------------------------------------------------------------------
+
+
+def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``scale = max |row| / 127``, ``code = round(x * 127 / max |row|)``.  A row of zeros: scale 0, codes 0; a row
+    with a NaN or an infinity: scale NaN, codes 0."""
+    x = x.float()
+    top = x.abs().amax(dim=1, keepdim=True)
+    finite = torch.isfinite(top)
+    # the smallest rows are lifted by 2^64 first: 127 / top would overflow
+    pre = torch.where(top < 2.0 ** -62, torch.full_like(top, 2.0 ** 64), torch.ones_like(top))
+    inv = torch.where(finite & (top > 0), 127.0 / (top * pre), torch.zeros_like(top))
+    codes = torch.where(finite, torch.round(x * pre * inv), torch.zeros_like(x))
+    scale = torch.where(finite, top / 127.0, torch.full_like(top, math.nan))
+    return codes.to(torch.int8), scale[:, 0]
+
+
+def dequantize_rows(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    return (q.float() * scale[:, None]).to(dtype)
+
+
+def add_rms_norm_int8(x: torch.Tensor, weight: Optional[torch.Tensor], residual: Optional[torch.Tensor],
+                      eps: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(codes, scales, h)`` of ``h = x + residual``, ``y = h * weight / sqrt(mean(h^2) + eps)``."""
+    h = x.float() if residual is None else x.float() + residual.float()
+    # squares and their mean in 64 bits: no row is too large or too small for them
+    rs = 1.0 / torch.sqrt(h.double().square().mean(dim=1, keepdim=True) + eps)
+    y = torch.where(h == 0, torch.zeros_like(h), (h.double() * rs).float())
+    y = torch.where(torch.isfinite(h).all(dim=1, keepdim=True), y, torch.full_like(y, math.nan))
+    q, scale = quantize_rows(y if weight is None else y * weight.float())
+    return q, scale, h.to(x.dtype)
+
+
+def linear_int8(q: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                bias: Optional[torch.Tensor], activation: str, dtype: torch.dtype) -> torch.Tensor:
+    """``act((q @ weight.T) * scale * weight_scale + bias)``; the sums are exact (64-bit floats hold them)."""
+    y = (q.double() @ weight.double().t()).float() * scale[:, None] * weight_scale
+    if bias is not None:
+        y = y + bias
+    return {"none": y, "relu": torch.relu(y), "tanh": torch.tanh(y)}[activation].to(dtype)
