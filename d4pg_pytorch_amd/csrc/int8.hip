@@ -14,6 +14,7 @@
 //  * A row that holds a NaN or an infinity gets scale NaN and codes 0: whatever reads it gets NaN, never a number.
 //  * A row of zeros gets scale 0 and codes 0.
 #include "common.h"
+#include <type_traits>
 
 enum { F_FP32 = 0, F_BF16 = 1, F_FP16 = 2, F_NONE = -1 };
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_TANH = 2 };
@@ -451,14 +452,27 @@ __device__ __forceinline__ void store4(T* out, const float (&v)[4], int left) {
             if (i < left) out[i] = (T)v[i];
     }
 }
-__device__ __forceinline__ void finish4(const LinearInt8Args& a, int m, int n, const i32x4 sum, float sm) {
+// What four neighbouring columns n .. n + 3 need besides their sums.
+struct Columns4 {
+    float scale[4], bias[4];
+};
+__device__ __forceinline__ Columns4 columns4(const LinearInt8Args& a, int n) {
+    Columns4 c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int ni = min(n + i, a.N - 1);
+        c.scale[i] = a.wscale[ni];
+        c.bias[i] = a.bias != nullptr ? a.bias[ni] : 0.f;
+    }
+    return c;
+}
+__device__ __forceinline__ void finish4(const LinearInt8Args& a, int m, int n, const i32x4 sum, float sm, const Columns4& c) {
     if (m >= a.M || n >= a.N) return;
     float v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int ni = min(n + i, a.N - 1);
-        v[i] = ((float)sum[i] * sm) * a.wscale[ni];
-        if (a.bias != nullptr) v[i] += a.bias[ni];
+        v[i] = ((float)sum[i] * sm) * c.scale[i];
+        if (a.bias != nullptr) v[i] += c.bias[i];
         v[i] = act_of(v[i], a.act);
     }
     const long long o = (long long)m * a.ld_out + n;
@@ -524,7 +538,7 @@ __global__ __launch_bounds__(64 * WAVES) void linear_int8_rows_kernel(const Line
 #pragma unroll
         for (int w = 1; w < WAVES; ++w) sum += part[w][u][lane];
         const int m = (tm * MT + u / NT) * 16 + c, n = (tn * NT + u % NT) * 16 + 4 * g;
-        finish4(a, m, n, sum, a.scale[min(m, a.M - 1)]);
+        finish4(a, m, n, sum, a.scale[min(m, a.M - 1)], columns4(a, n));
     }
 }
 
@@ -532,6 +546,135 @@ template <int MT, int NT, int WAVES>
 static void launch_linear_rows(const LinearInt8Args& a, hipStream_t stream) {
     const long long tiles = (long long)((a.M + 16 * MT - 1) / (16 * MT)) * ((a.N + 16 * NT - 1) / (16 * NT));
     hipLaunchKernelGGL((linear_int8_rows_kernel<MT, NT, WAVES>), dim3((unsigned)tiles), dim3(64 * WAVES), 0, stream, a);
+}
+
+// Many rows: a workgroup of 4 waves makes a tile of BM = 64 MI rows x BN = 64 NI columns, a wave 32 MI x 32 NI of it in
+// accumulators (v_mfma_i32_32x32x32_i8: lane 32 h + r holds 16 bytes of row r at k = 16 h; the weights are the A operand).
+//
+//  * Both tiles of 128 k lie in LDS twice.  Memory moves straight into LDS (16 bytes a lane, 8 rows of 128 bytes an
+//    instruction, no registers on the way); the move for step t + 2 starts as soon as every wave has read step t.
+//  * A wave reads the operands of a 32-k slice from LDS while it multiplies the slice before, across the border of two
+//    steps too: the one barrier of a step stands before its LAST slice, whose operands are in registers by then, so the
+//    matrix pipe has 16 products to run while the first reads of the next step return.
+//  * 16-byte pieces of a row are stored XOR (row % 8): the eight lanes of an LDS cycle then cover all banks.  The move
+//    writes LDS in lane order, so each lane fetches the piece that belongs at its place.
+//  * Rows beyond M or N repeat the last one and are not stored; pieces beyond K repeat the last one and are cleared in the
+//    activation operand of the last step.
+//  * Workgroups of one XCD (blockIdx % 8) take neighbouring tiles, 8 tile rows at a time, so that what they share is in
+//    their L2.
+enum { STEP_LOAD = 0, STEP_READ = 1, STEP_LAST = 2 };
+
+template <int MI, int NI>
+__device__ __forceinline__ void linear_tile(const LinearInt8Args& a, signed char* const lds) {
+    constexpr int BM = 64 * MI, BN = 64 * NI, TILE = (BM + BN) * 128, GROUP = 8;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave & 1, wn = wave >> 1, r = lane & 31, h = lane >> 5;
+
+    const int tiles_m = (a.M + BM - 1) / BM, tiles_n = (a.N + BN - 1) / BN, total = tiles_m * tiles_n;
+    const int xcd = blockIdx.x & 7, share = total >> 3, rest = total & 7;
+    const int id = (xcd < rest ? xcd * (share + 1) : rest * (share + 1) + (xcd - rest) * share) + (blockIdx.x >> 3);
+    const int width = GROUP * tiles_n, first = id / width * GROUP, in = id % width, rows = min(tiles_m - first, GROUP);
+    const int m0 = (first + in % rows) * BM, n0 = in / rows * BN;
+
+    const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc((void*)(a.q + (long long)m0 * a.ld_q), 0, 0x7fffffff, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w + (long long)n0 * a.ld_w), 0, 0x7fffffff, 0x00020000);
+    int oq[2 * MI], ow[2 * NI];                   // this lane's row of each move, in bytes from the tile's first row
+#pragma unroll
+    for (int i = 0; i < 2 * MI; ++i) oq[i] = min(wave * (BM / 4) + i * 8 + (lane >> 3), a.M - 1 - m0) * (int)a.ld_q;
+#pragma unroll
+    for (int i = 0; i < 2 * NI; ++i) ow[i] = min(wave * (BN / 4) + i * 8 + (lane >> 3), a.N - 1 - n0) * (int)a.ld_w;
+    const int piece = ((lane & 7) ^ (lane >> 3)) * 16, last = ((a.K - 1) >> 4) << 4;
+
+    auto load = [&](int t) {
+        const int k = min(t * 128 + piece, last);
+        signed char* const to = lds + (t & 1) * TILE;
+#pragma unroll
+        for (int i = 0; i < 2 * MI; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rq, (__attribute__((address_space(3))) void*)(to + (wave * (BM / 4) + i * 8) * 128), 16, oq[i] + k, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 2 * NI; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (__attribute__((address_space(3))) void*)(to + (BM + wave * (BN / 4) + i * 8) * 128), 16, ow[i] + k, 0, 0, 0);
+    };
+    i32x4 fx[2][MI], fw[2][NI];
+    auto read = [&](int t, int ks, int b) {
+        const signed char* const from = lds + (t & 1) * TILE + ((2 * ks + h) ^ (lane & 7)) * 16;
+#pragma unroll
+        for (int i = 0; i < MI; ++i) fx[b][i] = *reinterpret_cast<const i32x4*>(from + (wm * 32 * MI + i * 32 + r) * 128);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) fw[b][i] = *reinterpret_cast<const i32x4*>(from + (BM + wn * 32 * NI + i * 32 + r) * 128);
+    };
+    i32x16 acc[NI][MI] = {};
+    auto step = [&](int t, auto mode_c) {
+        constexpr int MODE = decltype(mode_c)::value;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            if (ks < 3) {
+                read(t, ks + 1, (ks + 1) & 1);
+            } else if (MODE != STEP_LAST) {
+                __syncthreads();                  // step t + 1 has arrived, step t has been read by every wave
+                read(t + 1, 0, 0);
+                if (MODE == STEP_LOAD) load(t + 2);
+            }
+            if (MODE == STEP_LAST) {
+                const i32x4 mask = below(t * 128 + ks * 32 + h * 16, a.K);
+#pragma unroll
+                for (int j = 0; j < MI; ++j) fx[ks & 1][j] &= mask;
+            }
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+#pragma unroll
+                for (int j = 0; j < MI; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[ks & 1][i], fx[ks & 1][j], acc[i][j], 0, 0, 0);
+        }
+    };
+    const int steps = (a.K + 127) >> 7;
+    load(0);
+    __syncthreads();
+    if (steps > 1) load(1);
+    read(0, 0, 0);
+    for (int t = 0; t < steps - 2; ++t) step(t, std::integral_constant<int, STEP_LOAD>());
+    if (steps > 1) step(steps - 2, std::integral_constant<int, STEP_READ>());
+    step(steps - 1, std::integral_constant<int, STEP_LAST>());
+
+    // Element 4 e + i of an accumulator is column 8 e + 4 h + i of its 32, row r.  32 rows of the wave at a time go through
+    // LDS (its own part of it; rows 16 bytes apart from a bank's multiple), so that a row's columns leave side by side.
+    constexpr int PITCH = 32 * NI + 4, LANES = 8 * NI;            // words of a row; lanes that write one row of 4 columns each
+    int* const stage = reinterpret_cast<int*>(lds) + wave * 32 * PITCH;
+    const int n = n0 + wn * 32 * NI + lane % LANES * 4;
+    const Columns4 col = columns4(a, n);
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < MI; ++j) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const i32x4 sum = {acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
+                *reinterpret_cast<i32x4*>(stage + r * PITCH + i * 32 + 8 * e + 4 * h) = sum;
+            }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int row = lane / LANES; row < 32; row += 64 / LANES) {
+            const int m = m0 + wm * 32 * MI + j * 32 + row;
+            const i32x4 sum = *reinterpret_cast<const i32x4*>(stage + row * PITCH + lane % LANES * 4);
+            finish4(a, m, n, sum, a.scale[min(m, a.M - 1)], col);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+template <int MI, int NI>
+__global__ __launch_bounds__(256, MI * NI > 8 ? 1 : 2) void linear_int8_tiles_kernel(const LinearInt8Args a) {
+    extern __shared__ __attribute__((aligned(128))) signed char tiles[];
+    linear_tile<MI, NI>(a, tiles);
+}
+
+template <int MI, int NI>
+static int launch_linear_tiles(const LinearInt8Args& a, hipStream_t stream) {
+    constexpr int LDS = 2 * (64 * MI + 64 * NI) * 128;
+    const long long tiles = (long long)((a.M + 64 * MI - 1) / (64 * MI)) * ((a.N + 64 * NI - 1) / (64 * NI));
+    if (tiles > 0x7fffffffll) return -7;
+    hipLaunchKernelGGL((linear_int8_tiles_kernel<MI, NI>), dim3((unsigned)tiles), dim3(256), LDS, stream, a);
+    return (int)hipGetLastError();
 }
 
 D4PG_API int d4pg_linear_int8(const LinearInt8Args* a, hipStream_t stream) {
@@ -543,6 +686,10 @@ D4PG_API int d4pg_linear_int8(const LinearInt8Args* a, hipStream_t stream) {
     if (((uintptr_t)a->q | (uintptr_t)a->w) & 15) return -5;
     if (a->dtype < F_FP32 || a->dtype > F_FP16 || a->act < ACT_NONE || a->act > ACT_TANH) return -6;
     if ((long long)((a->M + 15) / 16) * ((a->N + 15) / 16) > 0x7fffffffll) return -7;
+    // the tiles' offsets inside 256 rows are 32-bit
+    const bool near = 256 * (a->M > 1 ? a->ld_q : kp) + kp < 0x7fffffffll && 256 * (a->N > 1 ? a->ld_w : kp) + kp < 0x7fffffffll;
+    if (near && a->M >= 1024 && a->N >= 1024) return launch_linear_tiles<4, 4>(*a, stream);
+    if (near && a->M >= 128 && a->N >= 128) return launch_linear_tiles<2, 2>(*a, stream);
     if (a->M <= 16) launch_linear_rows<1, 1, 4>(*a, stream);
     else launch_linear_rows<2, 2, 4>(*a, stream);
     return (int)hipGetLastError();
