@@ -495,7 +495,9 @@ __device__ __forceinline__ i32x4 below(int k, int K) {
 // Few rows or small layers: a workgroup makes 16 MT rows x 16 NT columns, its WAVES waves split K and meet in LDS.
 // Operands go from memory to the matrix instruction's registers directly (v_mfma_i32_16x16x64_i8: lane 16 g + c holds
 // 16 bytes of row c at k = 16 g); the weights are the A operand, so that a lane ends with four neighbouring columns.
-template <int MT, int NT, int WAVES>
+// A wave issues the loads of U slices of 64 k before it multiplies the first: at these sizes the time is that of the
+// loads' way from memory.
+template <int MT, int NT, int WAVES, int U>
 __global__ __launch_bounds__(64 * WAVES) void linear_int8_rows_kernel(const LinearInt8Args a) {
     __shared__ i32x4 part[WAVES][MT * NT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -510,23 +512,31 @@ __global__ __launch_bounds__(64 * WAVES) void linear_int8_rows_kernel(const Line
     for (int i = 0; i < NT; ++i) wp[i] = a.w + (long long)min((tn * NT + i) * 16 + c, a.N - 1) * a.ld_w;
     const int last = ((a.K - 1) >> 4) << 4;      // the last 16 bytes of a row that hold a code
     i32x4 acc[MT][NT] = {};
-    // step s of the wave covers k = 64 (wave + s WAVES): neighbouring waves read neighbouring bytes
-    for (int k0 = 64 * wave; k0 < a.K; k0 += 64 * WAVES) {
-        const int k = k0 + 16 * g, kc = min(k, last);
-        i32x4 x[MT], w[NT];
+    // slice s of the wave covers k = 64 (wave + s WAVES): neighbouring waves read neighbouring bytes
+    for (int k0 = 64 * wave; k0 < a.K; k0 += 64 * WAVES * U) {
+        i32x4 x[U][MT], w[U][NT];
 #pragma unroll
-        for (int i = 0; i < NT; ++i) w[i] = *reinterpret_cast<const i32x4*>(wp[i] + kc);
+        for (int u = 0; u < U; ++u) {
+            const int kc = min(k0 + 64 * WAVES * u + 16 * g, last);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) x[i] = *reinterpret_cast<const i32x4*>(xp[i] + kc);
-        if (k0 + 64 > a.K) {
-            const i32x4 m = below(k, a.K);
+            for (int i = 0; i < NT; ++i) w[u][i] = *reinterpret_cast<const i32x4*>(wp[i] + kc);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) x[i] &= m;
+            for (int i = 0; i < MT; ++i) x[u][i] = *reinterpret_cast<const i32x4*>(xp[i] + kc);
+        }
+        if (k0 + 64 * WAVES * (U - 1) + 64 > a.K) {      // what lies beyond K repeats the last bytes: cleared on one side
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const i32x4 mask = below(k0 + 64 * WAVES * u + 16 * g, a.K);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) x[u][i] &= mask;
+            }
         }
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[j], x[i], acc[i][j], 0, 0, 0);
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u][j], x[u][i], acc[i][j], 0, 0, 0);
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -542,33 +552,40 @@ __global__ __launch_bounds__(64 * WAVES) void linear_int8_rows_kernel(const Line
     }
 }
 
-template <int MT, int NT, int WAVES>
-static void launch_linear_rows(const LinearInt8Args& a, hipStream_t stream) {
+template <int MT, int NT, int WAVES, int U>
+static int launch_linear_rows(const LinearInt8Args& a, hipStream_t stream) {
     const long long tiles = (long long)((a.M + 16 * MT - 1) / (16 * MT)) * ((a.N + 16 * NT - 1) / (16 * NT));
-    hipLaunchKernelGGL((linear_int8_rows_kernel<MT, NT, WAVES>), dim3((unsigned)tiles), dim3(64 * WAVES), 0, stream, a);
+    hipLaunchKernelGGL((linear_int8_rows_kernel<MT, NT, WAVES, U>), dim3((unsigned)tiles), dim3(64 * WAVES), 0, stream, a);
+    return (int)hipGetLastError();
 }
 
-// Many rows: a workgroup of 4 waves makes a tile of BM = 64 MI rows x BN = 64 NI columns, a wave 32 MI x 32 NI of it in
-// accumulators (v_mfma_i32_32x32x32_i8: lane 32 h + r holds 16 bytes of row r at k = 16 h; the weights are the A operand).
+// Many rows: a workgroup of WM x WN waves makes a tile of BM = 32 MI WM rows x BN = 32 NI WN columns, a wave 32 MI x 32 NI
+// of it in accumulators (v_mfma_i32_32x32x32_i8: lane 32 h + r holds 16 bytes of row r at k = 16 h; the weights are the A
+// operand).
 //
 //  * Both tiles of 128 k lie in LDS twice.  Memory moves straight into LDS (16 bytes a lane, 8 rows of 128 bytes an
 //    instruction, no registers on the way); the move for step t + 2 starts as soon as every wave has read step t.
 //  * A wave reads the operands of a 32-k slice from LDS while it multiplies the slice before, across the border of two
-//    steps too: the one barrier of a step stands before its LAST slice, whose operands are in registers by then, so the
-//    matrix pipe has 16 products to run while the first reads of the next step return.
-//  * 16-byte pieces of a row are stored XOR (row % 8): the eight lanes of an LDS cycle then cover all banks.  The move
-//    writes LDS in lane order, so each lane fetches the piece that belongs at its place.
+//    steps too: the one barrier of a step stands before its LAST slice, whose operands are in registers by then.
+//  * 16-byte pieces of a row are stored XOR (row / 2 % 8): the 16 lanes of an LDS cycle (256 bytes) then cover all banks
+//    (XOR row % 8 left every other cycle in conflict).  The move writes LDS in lane order, so each lane fetches the piece
+//    that belongs at its place.
 //  * Rows beyond M or N repeat the last one and are not stored; pieces beyond K repeat the last one and are cleared in the
 //    activation operand of the last step.
-//  * Workgroups of one XCD (blockIdx % 8) take neighbouring tiles, 8 tile rows at a time, so that what they share is in
-//    their L2.
+//  * Workgroups of one XCD (blockIdx % 8) take neighbouring tiles, 2048 rows of them at a time, so that what they share is
+//    in their L2 (moves alone, 8192^3 in tiles of 256: 247 us with 4 tile rows, 231 - 254 with 8, 300 with 16).
+//
+// What bounds it at 8192^3 (tiles of 256): power first - the matrix instruction alone does 4.9 P/s on zeros, 3.5 on random
+// codes, 3.1 - 3.2 with its LDS reads - then how well the rest hides behind it.  Moves alone take 231 us.  Waves a SIMD
+// decide the rest: 1 (waves of 128 x 128) 560 us, matrix pipe 52 % busy; 2 (128 x 64) 476; 4 (64 x 64) 464 us = 2.37 P/s.
 enum { STEP_LOAD = 0, STEP_READ = 1, STEP_LAST = 2 };
 
-template <int MI, int NI>
+template <int MI, int NI, int WM, int WN>
 __device__ __forceinline__ void linear_tile(const LinearInt8Args& a, signed char* const lds) {
-    constexpr int BM = 64 * MI, BN = 64 * NI, TILE = (BM + BN) * 128, GROUP = 8;
+    constexpr int BM = 32 * MI * WM, BN = 32 * NI * WN, TILE = (BM + BN) * 128, GROUP = 2048 / BM;
+    constexpr int MOVES = (BM + BN) / 8 / (WM * WN);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave & 1, wn = wave >> 1, r = lane & 31, h = lane >> 5;
+    const int wm = wave % WM, wn = wave / WM, r = lane & 31, h = lane >> 5;
 
     const int tiles_m = (a.M + BM - 1) / BM, tiles_n = (a.N + BN - 1) / BN, total = tiles_m * tiles_n;
     const int xcd = blockIdx.x & 7, share = total >> 3, rest = total & 7;
@@ -576,32 +593,31 @@ __device__ __forceinline__ void linear_tile(const LinearInt8Args& a, signed char
     const int width = GROUP * tiles_n, first = id / width * GROUP, in = id % width, rows = min(tiles_m - first, GROUP);
     const int m0 = (first + in % rows) * BM, n0 = in / rows * BN;
 
-    const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc((void*)(a.q + (long long)m0 * a.ld_q), 0, 0x7fffffff, 0x00020000);
-    const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w + (long long)n0 * a.ld_w), 0, 0x7fffffff, 0x00020000);
-    int oq[2 * MI], ow[2 * NI];                   // this lane's row of each move, in bytes from the tile's first row
+    // the wave's rows in LDS: the activations' are 0 .. BM - 1, the weights' follow
+    static_assert(BM / 8 % MOVES == 0 && MOVES % 2 == 0, "a wave moves rows of one operand, 16 at a time");
+    const int row0 = wave * MOVES * 8;
+    const bool acts = row0 < BM;
+    const signed char* const from = acts ? a.q + (long long)m0 * a.ld_q : a.w + (long long)n0 * a.ld_w;
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)from, 0, 0x7fffffff, 0x00020000);
+    const int ld = (int)(acts ? a.ld_q : a.ld_w), bottom = acts ? a.M - 1 - m0 : a.N - 1 - n0, base = acts ? row0 : row0 - BM;
+    int off[MOVES];                               // this lane's row of each move, in bytes from the tile's first row
 #pragma unroll
-    for (int i = 0; i < 2 * MI; ++i) oq[i] = min(wave * (BM / 4) + i * 8 + (lane >> 3), a.M - 1 - m0) * (int)a.ld_q;
-#pragma unroll
-    for (int i = 0; i < 2 * NI; ++i) ow[i] = min(wave * (BN / 4) + i * 8 + (lane >> 3), a.N - 1 - n0) * (int)a.ld_w;
-    const int piece = ((lane & 7) ^ (lane >> 3)) * 16, last = ((a.K - 1) >> 4) << 4;
-
+    for (int i = 0; i < MOVES; ++i) off[i] = min(base + i * 8 + (lane >> 3), bottom) * ld;
+    const int piece[2] = {((lane & 7) ^ (lane >> 4)) * 16, ((lane & 7) ^ (4 + (lane >> 4))) * 16}, last = ((a.K - 1) >> 4) << 4;
     auto load = [&](int t) {
-        const int k = min(t * 128 + piece, last);
-        signed char* const to = lds + (t & 1) * TILE;
+        const int k[2] = {min(t * 128 + piece[0], last), min(t * 128 + piece[1], last)};
+        signed char* const to = lds + (t & 1) * TILE + row0 * 128;
 #pragma unroll
-        for (int i = 0; i < 2 * MI; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rq, (__attribute__((address_space(3))) void*)(to + (wave * (BM / 4) + i * 8) * 128), 16, oq[i] + k, 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 2 * NI; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (__attribute__((address_space(3))) void*)(to + (BM + wave * (BN / 4) + i * 8) * 128), 16, ow[i] + k, 0, 0, 0);
+        for (int i = 0; i < MOVES; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(to + i * 1024), 16, off[i] + k[i & 1], 0, 0, 0);
     };
     i32x4 fx[2][MI], fw[2][NI];
     auto read = [&](int t, int ks, int b) {
-        const signed char* const from = lds + (t & 1) * TILE + ((2 * ks + h) ^ (lane & 7)) * 16;
+        const signed char* const at = lds + (t & 1) * TILE + ((2 * ks + h) ^ ((lane >> 1) & 7)) * 16;
 #pragma unroll
-        for (int i = 0; i < MI; ++i) fx[b][i] = *reinterpret_cast<const i32x4*>(from + (wm * 32 * MI + i * 32 + r) * 128);
+        for (int i = 0; i < NI; ++i) fw[b][i] = *reinterpret_cast<const i32x4*>(at + (BM + wn * 32 * NI + i * 32 + r) * 128);
 #pragma unroll
-        for (int i = 0; i < NI; ++i) fw[b][i] = *reinterpret_cast<const i32x4*>(from + (BM + wn * 32 * NI + i * 32 + r) * 128);
+        for (int i = 0; i < MI; ++i) fx[b][i] = *reinterpret_cast<const i32x4*>(at + (wm * 32 * MI + i * 32 + r) * 128);
     };
     i32x16 acc[NI][MI] = {};
     auto step = [&](int t, auto mode_c) {
@@ -662,19 +678,51 @@ __device__ __forceinline__ void linear_tile(const LinearInt8Args& a, signed char
     }
 }
 
-template <int MI, int NI>
-__global__ __launch_bounds__(256, MI * NI > 8 ? 1 : 2) void linear_int8_tiles_kernel(const LinearInt8Args a) {
+template <int MI, int NI, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, WM * WN / 4 * (MI * NI * WM * WN > 32 ? 1 : 2)) void linear_int8_tiles_kernel(const LinearInt8Args a) {
     extern __shared__ __attribute__((aligned(128))) signed char tiles[];
-    linear_tile<MI, NI>(a, tiles);
+    linear_tile<MI, NI, WM, WN>(a, tiles);
 }
 
-template <int MI, int NI>
+template <int MI, int NI, int WM, int WN>
 static int launch_linear_tiles(const LinearInt8Args& a, hipStream_t stream) {
-    constexpr int LDS = 2 * (64 * MI + 64 * NI) * 128;
-    const long long tiles = (long long)((a.M + 64 * MI - 1) / (64 * MI)) * ((a.N + 64 * NI - 1) / (64 * NI));
+    constexpr int BM = 32 * MI * WM, BN = 32 * NI * WN, TILES = 2 * (BM + BN) * 128, STAGE = WM * WN * 32 * (32 * NI + 4) * 4;
+    constexpr int LDS = TILES > STAGE ? TILES : STAGE;
+    const long long tiles = (long long)((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN);
     if (tiles > 0x7fffffffll) return -7;
-    hipLaunchKernelGGL((linear_int8_tiles_kernel<MI, NI>), dim3((unsigned)tiles), dim3(256), LDS, stream, a);
+    hipLaunchKernelGGL((linear_int8_tiles_kernel<MI, NI, WM, WN>), dim3((unsigned)tiles), dim3(64 * WM * WN), LDS, stream, a);
     return (int)hipGetLastError();
+}
+
+// Which kernel.  Tiles are taken from the largest size that still gives most of the 256 CUs one; below 128 tiles of 64 x 64
+// (256 where K is short: a tile then ends before its moves have paid) the rows kernel, whose workgroups split K instead.
+// Measured on an MI355X, us (graph of 20 calls, median), the other choice behind the /:
+//     256 x 256, 16 waves    2048 x 8192 x 8192 (256 tiles)  132 / 158 (128 x 128)    2048 x 4096 x 4096 (128)  54 / 45
+//     128 x 128, 8 waves     4096 x 1024 x 1024 (256)        13.8 / 13.4 (64 x 64)    512 x 4096 x 4096 (128)   24.8 / 18.9
+//     64 x 64, 4 waves       256 x 4096 x 4096 (256)         12.7 / 25 (rows)         512 x 1024 x 1024 (128)   6.7 / 6.3
+// Between the row kernels the number of 16 x 16 tiles decides: as many columns and rows a workgroup as leave 200 - 400
+// workgroups (256 x 400 x 400: 3.7 with 2 x 1 tiles, 4.0 with 1 x 1, 4.2 with 2 x 2; 512 x 1024 x 1024: 6.3 with 4 x 2, 6.9
+// with 2 x 2, 8.6 with 2 x 1; 1 x 16384 x 4096: 13.9 with 1 x 4, 15.2 with 1 x 1), and K is dealt to 16 waves where it is long
+// and the workgroups are few (1 x 4096 x 4096: 5.6 with 16 waves, 6.6 with 4; 1 x 1333 x 2001: 4.4 and 3.6).
+static int launch_linear(const LinearInt8Args& a, long long kp, hipStream_t stream) {
+    auto tiles = [&](int side) { return (long long)((a.M + side - 1) / side) * ((a.N + side - 1) / side); };
+    // the tile kernel's offsets inside 256 rows are 32-bit
+    if (256 * (a.M > 1 ? a.ld_q : kp) + kp < 0x7fffffffll && 256 * (a.N > 1 ? a.ld_w : kp) + kp < 0x7fffffffll) {
+        if (tiles(256) >= 192) return launch_linear_tiles<2, 2, 4, 4>(a, stream);
+        if (tiles(128) >= 192) return launch_linear_tiles<2, 1, 2, 4>(a, stream);
+        if (tiles(64) >= (a.K <= 1024 ? 256 : 128)) return launch_linear_tiles<1, 1, 2, 2>(a, stream);
+    }
+    const long long t = tiles(16);
+    if (a.M <= 16) {
+        if (t >= 768) return launch_linear_rows<1, 4, 4, 2>(a, stream);
+        if (t <= 256 && a.K >= 4096) return launch_linear_rows<1, 1, 16, 4>(a, stream);
+        return launch_linear_rows<1, 1, 4, 4>(a, stream);
+    }
+    if (t <= 320) return launch_linear_rows<1, 1, 4, 4>(a, stream);
+    if (t <= 640) return launch_linear_rows<2, 1, 8, 2>(a, stream);
+    if (t <= 1536) return launch_linear_rows<2, 2, 4, 4>(a, stream);
+    if (a.M <= 32) return launch_linear_rows<2, 4, 4, 2>(a, stream);
+    return launch_linear_rows<4, 2, 8, 2>(a, stream);
 }
 
 D4PG_API int d4pg_linear_int8(const LinearInt8Args* a, hipStream_t stream) {
@@ -686,13 +734,7 @@ D4PG_API int d4pg_linear_int8(const LinearInt8Args* a, hipStream_t stream) {
     if (((uintptr_t)a->q | (uintptr_t)a->w) & 15) return -5;
     if (a->dtype < F_FP32 || a->dtype > F_FP16 || a->act < ACT_NONE || a->act > ACT_TANH) return -6;
     if ((long long)((a->M + 15) / 16) * ((a->N + 15) / 16) > 0x7fffffffll) return -7;
-    // the tiles' offsets inside 256 rows are 32-bit
-    const bool near = 256 * (a->M > 1 ? a->ld_q : kp) + kp < 0x7fffffffll && 256 * (a->N > 1 ? a->ld_w : kp) + kp < 0x7fffffffll;
-    if (near && a->M >= 1024 && a->N >= 1024) return launch_linear_tiles<4, 4>(*a, stream);
-    if (near && a->M >= 128 && a->N >= 128) return launch_linear_tiles<2, 2>(*a, stream);
-    if (a->M <= 16) launch_linear_rows<1, 1, 4>(*a, stream);
-    else launch_linear_rows<2, 2, 4>(*a, stream);
-    return (int)hipGetLastError();
+    return launch_linear(*a, kp, stream);
 }
 
 D4PG_SIZEOF(QuantRowsArgs)
