@@ -456,29 +456,36 @@ __device__ __forceinline__ void store4(T* out, const float (&v)[4], int left) {
 struct Columns4 {
     float scale[4], bias[4];
 };
-__device__ __forceinline__ Columns4 columns4(const LinearInt8Args& a, int n) {
+__device__ __forceinline__ Columns4 columns4(const float* wscale, const float* bias, int n, int N) {
     Columns4 c;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int ni = min(n + i, a.N - 1);
-        c.scale[i] = a.wscale[ni];
-        c.bias[i] = a.bias != nullptr ? a.bias[ni] : 0.f;
+        const int ni = min(n + i, N - 1);
+        c.scale[i] = wscale[ni];
+        c.bias[i] = bias != nullptr ? bias[ni] : 0.f;
     }
     return c;
+}
+// act(sum * s * t + b) of four columns.  ONE definition, contraction off: every kernel below rounds alike.
+__device__ __forceinline__ void values4(float (&v)[4], const i32x4 sum, float sm, const Columns4& c, bool biased, int act) {
+#pragma clang fp contract(off)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[i] = ((float)sum[i] * sm) * c.scale[i];
+        if (biased) v[i] += c.bias[i];
+        v[i] = act_of(v[i], act);
+    }
+}
+__device__ __forceinline__ void store_values4(void* out, long long at, int dtype, const float (&v)[4], int left) {
+    if (dtype == F_FP32) store4(reinterpret_cast<float*>(out) + at, v, left);
+    else if (dtype == F_BF16) store4(reinterpret_cast<__bf16*>(out) + at, v, left);
+    else store4(reinterpret_cast<_Float16*>(out) + at, v, left);
 }
 __device__ __forceinline__ void finish4(const LinearInt8Args& a, int m, int n, const i32x4 sum, float sm, const Columns4& c) {
     if (m >= a.M || n >= a.N) return;
     float v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[i] = ((float)sum[i] * sm) * c.scale[i];
-        if (a.bias != nullptr) v[i] += c.bias[i];
-        v[i] = act_of(v[i], a.act);
-    }
-    const long long o = (long long)m * a.ld_out + n;
-    if (a.dtype == F_FP32) store4(reinterpret_cast<float*>(a.out) + o, v, a.N - n);
-    else if (a.dtype == F_BF16) store4(reinterpret_cast<__bf16*>(a.out) + o, v, a.N - n);
-    else store4(reinterpret_cast<_Float16*>(a.out) + o, v, a.N - n);
+    values4(v, sum, sm, c, a.bias != nullptr, a.act);
+    store_values4(a.out, (long long)m * a.ld_out + n, a.dtype, v, a.N - n);
 }
 
 // All ones in the bytes k .. k + 15 that lie below K.
@@ -548,7 +555,7 @@ __global__ __launch_bounds__(64 * WAVES) void linear_int8_rows_kernel(const Line
 #pragma unroll
         for (int w = 1; w < WAVES; ++w) sum += part[w][u][lane];
         const int m = (tm * MT + u / NT) * 16 + c, n = (tn * NT + u % NT) * 16 + 4 * g;
-        finish4(a, m, n, sum, a.scale[min(m, a.M - 1)], columns4(a, n));
+        finish4(a, m, n, sum, a.scale[min(m, a.M - 1)], columns4(a.wscale, a.bias, n, a.N));
     }
 }
 
@@ -656,7 +663,7 @@ __device__ __forceinline__ void linear_tile(const LinearInt8Args& a, signed char
     constexpr int PITCH = 32 * NI + 4, LANES = 8 * NI;            // words of a row; lanes that write one row of 4 columns each
     int* const stage = reinterpret_cast<int*>(lds) + wave * 32 * PITCH;
     const int n = n0 + wn * 32 * NI + lane % LANES * 4;
-    const Columns4 col = columns4(a, n);
+    const Columns4 col = columns4(a.wscale, a.bias, n, a.N);
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < MI; ++j) {
@@ -714,9 +721,9 @@ static int launch_linear(const LinearInt8Args& a, long long kp, hipStream_t stre
     }
     const long long t = tiles(16);
     if (a.M <= 16) {
-        if (t >= 768) return launch_linear_rows<1, 4, 4, 2>(a, stream);
+        if (t >= 768) return launch_linear_rows<1, 4, 4, 1>(a, stream);
         if (t <= 256 && a.K >= 4096) return launch_linear_rows<1, 1, 16, 4>(a, stream);
-        return launch_linear_rows<1, 1, 4, 4>(a, stream);
+        return launch_linear_rows<1, 1, 4, 2>(a, stream);
     }
     if (t <= 320) return launch_linear_rows<1, 1, 4, 4>(a, stream);
     if (t <= 640) return launch_linear_rows<2, 1, 8, 2>(a, stream);
@@ -736,6 +743,251 @@ D4PG_API int d4pg_linear_int8(const LinearInt8Args* a, hipStream_t stream) {
     if ((long long)((a->M + 15) / 16) * ((a->N + 15) / 16) > 0x7fffffffll) return -7;
     return launch_linear(*a, kp, stream);
 }
+
+// ---------------------------------------------------------------------------------------------------------------
+// three layers on codes in one launch
+// ---------------------------------------------------------------------------------------------------------------
+// Everything but the weights is local to a row, so a workgroup of 16 waves takes 16 MT rows through the whole network with
+// their codes in LDS: quantise the input, then per layer the product (weights straight from L2 to registers,
+// v_mfma_i32_16x16x64_i8 with the weights as the A operand: lane 16 g + c ends with columns 4 g .. 4 g + 3 of row c), the
+// activation, the rows' largest magnitudes (LDS integer maxima: whatever the order, the same result) and the codes of the
+// next layer.  No hidden value leaves the CU.
+//
+// A layer whose columns make more than 8 tiles of 16 deals them to the waves (TPW each); a narrower one deals K, the waves
+// of a tile meeting in LDS integer additions.  Codes lie in LDS in rows 16 bytes apart from a multiple of 64, zero from the
+// layer's width up to it: the 16 lanes of an LDS cycle cover all banks, and what the weights hold beyond K meets zeros.
+struct Mlp3Int8Args {
+    const void* x;                 // [M, width[0]] rows of ld_x elements
+    void* out;                     // [M, width[3]] rows of ld_out elements
+    const signed char* w[3];       // [width[i + 1], width[i]] codes, rows of ld_w[i] bytes
+    const float* wscale[3];
+    const float* bias[3];          // or null
+    long long ld_x, ld_out, ld_w[3];
+    int M, width[4];
+    int xdtype, dtype, act;        // F_* of x and out; ACT_* of the last layer (the others: ReLU)
+    int pad_;
+    int pitch, split;              // bytes of a row of codes in LDS, words of the split layers' sums (set by the host entry)
+};
+constexpr int MLP_WAVES = 16;
+
+__device__ __forceinline__ float load_any(const void* p, int dtype, long long i) {
+    if (dtype == F_FP32) return load1<float>(p, i);
+    if (dtype == F_BF16) return load1<__bf16>(p, i);
+    return load1<_Float16>(p, i);
+}
+
+// The products of NT column tiles n0[j] .. n0[j] + 15 with the workgroup's rows, over slices of 64 k from k0 on, `step`
+// apart.  The loads of U slices are issued before the first product.
+template <int NT, int MT, int U>
+__device__ __forceinline__ void mlp_product(i32x4 (&acc)[NT][MT], const signed char* w, long long ld, int N, int K, const int (&n0)[NT],
+                                            const signed char* codes, int pitch, int k0, int step) {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, last = ((K - 1) >> 4) << 4;
+    const signed char* wp[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) wp[j] = w + (long long)min(n0[j] + c, N - 1) * ld;
+    const signed char* const xp = codes + c * pitch + 16 * g;
+    for (int k = k0; k < K; k += step * U) {
+        i32x4 wf[U][NT];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) wf[u][j] = *reinterpret_cast<const i32x4*>(wp[j] + min(k + u * step + 16 * g, last));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (k + u * step >= K) break;        // the same for the wave
+            i32x4 xf[MT];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) xf[i] = *reinterpret_cast<const i32x4*>(xp + i * 16 * pitch + k + u * step);
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int i = 0; i < MT; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u][j], xf[i], acc[j][i], 0, 0, 0);
+        }
+    }
+}
+
+// Codes of row r, columns n .. n + 3 of one lane's values.
+__device__ __forceinline__ void mlp_codes(signed char* codes, int pitch, int r, int n, int N, const float (&v)[4], const RowCode& rc) {
+    unsigned b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = n + i < N ? code_bits(v[i], rc) & rc.keep : 0u;
+    *reinterpret_cast<unsigned*>(codes + r * pitch + n) = pack4(b[0], b[1], b[2], b[3]);
+}
+
+template <int TPW, int MT>
+__global__ __launch_bounds__(64 * MLP_WAVES) void mlp3_int8_kernel(const Mlp3Int8Args a) {
+    extern __shared__ __attribute__((aligned(128))) signed char mem[];
+    constexpr int ROWS = 16 * MT, U = TPW * MT >= 16 ? 1 : (TPW * MT >= 8 ? 2 : 4);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+    const int m0 = blockIdx.x * ROWS, pitch = a.pitch;
+    signed char* const codes[2] = {mem, mem + ROWS * pitch};
+    int* const sums = reinterpret_cast<int*>(mem + 2 * ROWS * pitch);
+    unsigned* const top = reinterpret_cast<unsigned*>(sums + a.split);       // [3][ROWS] largest magnitudes, as bits
+
+    for (int i = threadIdx.x; i < a.split; i += 64 * MLP_WAVES) sums[i] = 0;
+    for (int i = threadIdx.x; i < 3 * ROWS; i += 64 * MLP_WAVES) top[i] = 0u;
+    __syncthreads();
+    {
+        const int S = a.width[0], padded = (S + 63) & ~63;
+        for (int r = wave; r < ROWS; r += MLP_WAVES) {
+            const long long row = (long long)min(m0 + r, a.M - 1) * a.ld_x;
+            unsigned t = 0;
+            for (int k = lane; k < S; k += 64) t = max(t, abs_bits(load_any(a.x, a.xdtype, row + k)));
+            t = wave_umax(t);
+            if (lane == 0) top[r] = t;
+            const RowCode rc = row_code(t);
+            for (int k = lane; k < padded; k += 64)
+                codes[0][r * pitch + k] = k < S ? (signed char)(code_bits(load_any(a.x, a.xdtype, row + k), rc) & rc.keep) : 0;
+        }
+    }
+    __syncthreads();
+    for (int layer = 0; layer < 3; ++layer) {
+        const int K = a.width[layer], N = a.width[layer + 1], tiles = (N + 15) >> 4;
+        const signed char* const w = a.w[layer];
+        const float* const wscale = a.wscale[layer];
+        const float* const bias = a.bias[layer];
+        const signed char* const in = codes[layer & 1];
+        signed char* const next = codes[(layer & 1) ^ 1];
+        const int act = layer < 2 ? ACT_RELU : a.act;
+        const unsigned* const top_in = top + layer * ROWS;
+        // zeros from the layer's width up to the next slice (whole tiles write their own)
+        if (layer < 2)
+            for (int i = threadIdx.x; i < ROWS * 4; i += 64 * MLP_WAVES) {
+                const int n = (N & ~63) + 16 * (i & 3);
+                if ((N & 63) && n >= 16 * tiles) *reinterpret_cast<i32x4*>(next + (i >> 2) * pitch + n) = i32x4{0, 0, 0, 0};
+            }
+        if (tiles <= MLP_WAVES / 2) {
+            // few columns: the waves of a tile share K
+            const int lanes_of_tiles = tiles <= 1 ? 1 : (tiles <= 2 ? 2 : (tiles <= 4 ? 4 : 8)), parts = MLP_WAVES / lanes_of_tiles;
+            const int tile = wave & (lanes_of_tiles - 1), part = wave / lanes_of_tiles;
+            int* const sum = sums + (tile * MT * 64 + lane) * 4;
+            if (tile < tiles) {
+                i32x4 acc[1][MT] = {};
+                const int n0[1] = {tile * 16};
+                mlp_product<1, MT, 4>(acc, w, a.ld_w[layer], N, K, n0, in, pitch, 64 * part, 64 * parts);
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) atomicAdd(sum + i * 256 + e, acc[0][i][e]);
+            }
+            __syncthreads();
+            // units (tile, i): at most 8 MT of them, MT / 2 a wave
+            float v[(MT + 1) / 2][4];
+#pragma unroll
+            for (int u = 0; u < (MT + 1) / 2; ++u) {
+                const int unit = wave + u * MLP_WAVES, t = unit / MT, i = unit % MT, n = 16 * t + 4 * g, r = 16 * i + c;
+                if (t >= tiles) continue;
+                int* const from = sums + (unit * 64 + lane) * 4;
+                const i32x4 s = *reinterpret_cast<const i32x4*>(from);
+                *reinterpret_cast<i32x4*>(from) = i32x4{0, 0, 0, 0};           // for the next layer that needs them
+                values4(v[u], s, row_code(top_in[r]).scale, columns4(wscale, bias, n, N), bias != nullptr, act);
+                if (layer == 2) {
+                    if (m0 + r < a.M && n < N) store_values4(a.out, (long long)(m0 + r) * a.ld_out + n, a.dtype, v[u], N - n);
+                } else {
+                    unsigned m = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) m = max(m, n + e < N ? abs_bits(v[u][e]) : 0u);
+                    atomicMax(top + (layer + 1) * ROWS + r, m);
+                }
+            }
+            if (layer < 2) {
+                __syncthreads();
+#pragma unroll
+                for (int u = 0; u < (MT + 1) / 2; ++u) {
+                    const int unit = wave + u * MLP_WAVES, t = unit / MT, i = unit % MT, n = 16 * t + 4 * g, r = 16 * i + c;
+                    if (t < tiles) mlp_codes(next, pitch, r, n, N, v[u], row_code(top[(layer + 1) * ROWS + r]));
+                }
+            }
+        } else {
+            i32x4 acc[TPW][MT] = {};
+            int n0[TPW];
+#pragma unroll
+            for (int j = 0; j < TPW; ++j) n0[j] = 16 * (wave + j * MLP_WAVES);
+            mlp_product<TPW, MT, U>(acc, w, a.ld_w[layer], N, K, n0, in, pitch, 0, 64);
+            float v[TPW][MT][4];
+            unsigned m[MT] = {};
+#pragma unroll
+            for (int j = 0; j < TPW; ++j) {
+                const int n = n0[j] + 4 * g;
+                const Columns4 col = columns4(wscale, bias, n, N);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    const int r = 16 * i + c;
+                    values4(v[j][i], acc[j][i], row_code(top_in[r]).scale, col, bias != nullptr, act);
+                    if (layer == 2) {
+                        if (m0 + r < a.M && n < N) store_values4(a.out, (long long)(m0 + r) * a.ld_out + n, a.dtype, v[j][i], N - n);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) m[i] = max(m[i], n + e < N ? abs_bits(v[j][i][e]) : 0u);
+                    }
+                }
+            }
+            if (layer < 2) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    unsigned t = m[i];
+                    t = max(t, (unsigned)__shfl_xor((int)t, 16, 64));
+                    t = max(t, (unsigned)__shfl_xor((int)t, 32, 64));
+                    if (g == 0) atomicMax(top + (layer + 1) * ROWS + 16 * i + c, t);
+                }
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    const RowCode rc = row_code(top[(layer + 1) * ROWS + 16 * i + c]);
+#pragma unroll
+                    for (int j = 0; j < TPW; ++j)
+                        if (n0[j] < N) mlp_codes(next, pitch, 16 * i + c, n0[j] + 4 * g, N, v[j][i], rc);
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+template <int TPW, int MT>
+static int launch_mlp3(const Mlp3Int8Args& a, int lds, hipStream_t stream) {
+    hipLaunchKernelGGL((mlp3_int8_kernel<TPW, MT>), dim3((unsigned)((a.M + 16 * MT - 1) / (16 * MT))), dim3(64 * MLP_WAVES), lds, stream, a);
+    return (int)hipGetLastError();
+}
+template <int TPW>
+static int launch_mlp3_rows(const Mlp3Int8Args& a, int mt, int lds, hipStream_t stream) {
+    return mt == 1 ? launch_mlp3<TPW, 1>(a, lds, stream) : launch_mlp3<TPW, 2>(a, lds, stream);
+}
+
+// 0: enqueued; 1: outside this kernel's range (nothing was enqueued); < 0: bad arguments.
+D4PG_API int d4pg_mlp3_int8(Mlp3Int8Args* a, hipStream_t stream) {
+    if (a->M < 1 || a->x == nullptr || a->out == nullptr || a->ld_out < a->width[3]) return -1;
+    if (a->dtype < F_FP32 || a->dtype > F_FP16 || a->xdtype < F_FP32 || a->xdtype > F_FP16) return -6;
+    if (a->act < ACT_NONE || a->act > ACT_TANH) return -6;
+    int widest = 0, wide_out = 0, few = 0;
+    for (int i = 0; i < 4; ++i) {
+        if (a->width[i] < 1) return -1;
+        if (i < 3 && a->width[i] > widest) widest = a->width[i];
+    }
+    for (int i = 0; i < 3; ++i) {
+        const long long kp = (a->width[i] + 15) & ~15;
+        if (a->w[i] == nullptr || a->wscale[i] == nullptr) return -2;
+        if (((uintptr_t)a->w[i] & 15) || (a->width[i + 1] > 1 && ((a->ld_w[i] & 15) || a->ld_w[i] < kp))) return -3;
+        const int tiles = (a->width[i + 1] + 15) / 16;
+        if (tiles > wide_out) wide_out = tiles;
+        if (tiles <= MLP_WAVES / 2 && tiles > few) few = tiles;
+    }
+    if (widest > 2048 || wide_out > 128) return 1;
+    a->pitch = ((widest + 63) & ~63) + 16;
+    int mt = a->pad_;
+    if (mt == 0) mt = a->M <= 2048 ? 1 : 2;
+    for (;; mt /= 2) {
+        a->split = few * mt * 256;
+        const int lds = 2 * 16 * mt * a->pitch + 4 * a->split + 3 * 16 * mt * 4;
+        if (lds > 160 * 1024) continue;
+        if (wide_out <= 16) return launch_mlp3_rows<1>(*a, mt, lds, stream);
+        if (wide_out <= 32) return launch_mlp3_rows<2>(*a, mt, lds, stream);
+        if (wide_out <= 64) return launch_mlp3_rows<4>(*a, mt, lds, stream);
+        return launch_mlp3_rows<8>(*a, mt, lds, stream);
+    }
+}
+
+D4PG_SIZEOF(Mlp3Int8Args)
 
 D4PG_SIZEOF(QuantRowsArgs)
 D4PG_SIZEOF(DequantRowsArgs)

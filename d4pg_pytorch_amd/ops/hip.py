@@ -392,6 +392,13 @@ class LinearInt8Args(C.Structure):
                 ("M", C.c_int), ("N", C.c_int), ("K", C.c_int), ("act", C.c_int), ("dtype", C.c_int), ("pad_", C.c_int)]
 
 
+class Mlp3Int8Args(C.Structure):
+    _fields_ = [("x", vp), ("out", vp), ("w", vp * 3), ("wscale", vp * 3), ("bias", vp * 3),
+                ("ld_x", C.c_longlong), ("ld_out", C.c_longlong), ("ld_w", C.c_longlong * 3),
+                ("M", C.c_int), ("width", C.c_int * 4), ("xdtype", C.c_int), ("dtype", C.c_int), ("act", C.c_int),
+                ("pad_", C.c_int), ("pitch", C.c_int), ("split", C.c_int)]
+
+
 class DevStateMirror(C.Structure):
     """Host mirror of ``struct DevState`` (csrc/common.h) for init / read-back."""
     _fields_ = [("step_done", C.c_longlong), ("step_cur", C.c_longlong),
@@ -493,6 +500,7 @@ def lib() -> C.CDLL:
             ("d4pg_quant_rows", [C.POINTER(QuantRowsArgs), vp]),
             ("d4pg_dequant_rows", [C.POINTER(DequantRowsArgs), vp]),
             ("d4pg_linear_int8", [C.POINTER(LinearInt8Args), vp]),
+            ("d4pg_mlp3_int8", [C.POINTER(Mlp3Int8Args), vp]),
             ("d4pg_ipc_alloc", [C.c_size_t, C.POINTER(vp), C.c_char_p]),
             ("d4pg_ipc_open", [C.c_char_p, C.POINTER(vp)]),
             ("d4pg_ipc_close", [vp]),
@@ -566,6 +574,18 @@ def graph_kernel_nodes(graph: "torch.cuda.CUDAGraph") -> int:
     if n < 0:
         raise RuntimeError("hipGraphGetNodes failed")
     return int(n)
+
+
+def launch_on(name: str, args: C.Structure, index: int) -> int:
+    """Launch on the current stream of device ``index``, whichever device is current, and return the entry's code.  The
+    short way for single operators: asking torch for a ``Stream`` object costs as much as the launch."""
+    fn = getattr(lib(), name)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(C.byref(args), torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(C.byref(args), torch._C._cuda_getCurrentRawStream(index))
+    return rc
 
 
 def launch(name: str, args: C.Structure, stream: Optional[torch.cuda.Stream] = None) -> None:

@@ -29,6 +29,7 @@ _FLOATS = {torch.float32: H.F_FP32, torch.bfloat16: H.F_BF16, torch.float16: H.F
 _ACTS = {"none": H.ACT_NONE, "relu": H.ACT_RELU, "tanh": H.ACT_TANH}
 #: products of two codes are at most 128^2 in magnitude: sums of this many fit 32 bits
 MAX_K = 131071
+_F32, _I8 = torch.float32, torch.int8
 
 
 def _float_code(t: torch.Tensor, what: str) -> int:
@@ -45,40 +46,49 @@ def _out_code(dtype: torch.dtype) -> int:
     return code
 
 
-def _same_device(a: torch.Tensor, what: str, b: Optional[torch.Tensor]) -> None:
-    if b is not None and b.device != a.device:
-        raise ValueError(f"{what} is on {b.device}, not on {a.device}")
+def _act_code(activation: str) -> int:
+    code = _ACTS.get(activation)
+    if code is None:
+        raise ValueError(f"activation must be one of {sorted(_ACTS)}, not {activation!r}")
+    return code
 
 
-def _rows(x: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int]:
-    """``x[..., K]`` as ``[M, K]`` with neighbouring elements side by side, and ``M``, ``K``."""
-    if x.ndim < 1 or x.shape[-1] < 1:
+def _on(device: torch.device, what: str, t: torch.Tensor) -> None:
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, not on {device}")
+
+
+def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
+    """``x[..., K]`` as ``[M, K]`` with neighbouring elements side by side."""
+    if x.ndim != 2:
+        if x.ndim < 1 or x.shape[-1] < 1:
+            raise ValueError(f"{what} needs at least one column, not shape {tuple(x.shape)}")
+        x = x.reshape(-1, x.shape[-1])
+    K = x.shape[1]
+    if K < 1:
         raise ValueError(f"{what} needs at least one column, not shape {tuple(x.shape)}")
-    K = x.shape[-1]
-    x2 = x if x.ndim == 2 else x.reshape(-1, K)
-    if K > 1 and x2.stride(1) != 1:
-        x2 = x2.contiguous()
-    return x2, x2.shape[0], K
+    return x if K == 1 or x.stride(1) == 1 else x.contiguous()
 
 
-def _code_rows(q: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int, int]:
-    """Codes as ``[M, K]`` in rows the product can read 16 bytes at a time, with ``M``, ``K`` and the row stride."""
-    q2, M, K = _rows(q, what)
+def _code_rows(q: torch.Tensor, what: str) -> Tuple[torch.Tensor, int]:
+    """Codes as ``[M, K]`` in rows the product can read 16 bytes at a time, and the row stride."""
+    q = _rows(q, what)
+    M, K = q.shape
     kp = (K + 15) & ~15
-    ld = q2.stride(0) if M > 1 else kp
-    fits = q2.data_ptr() % 16 == 0 and ld % 16 == 0 and ld >= kp
+    ld = q.stride(0) if M > 1 else kp
+    fits = ld >= kp and ld % 16 == 0 and q.data_ptr() % 16 == 0
     if fits and kp != K:      # the bytes that fill the last row up must belong to the tensor's memory too
-        fits = q2.storage_offset() + (M - 1) * ld + kp <= q2.untyped_storage().nbytes()
-    if not fits:
-        buf = torch.empty(M, kp, dtype=torch.int8, device=q.device)
-        buf[:, :K] = q2
-        q2, ld = buf, kp
-    return q2, M, K, ld
+        fits = q.storage_offset() + (M - 1) * ld + kp <= q.untyped_storage().nbytes()
+    if fits:
+        return q, ld
+    buf = torch.empty(M, kp, dtype=_I8, device=q.device)
+    buf[:, :K] = q
+    return buf, kp
 
 
 def _new_codes(M: int, K: int, device) -> Tuple[torch.Tensor, int]:
     kp = (K + 15) & ~15
-    buf = torch.empty(M, kp, dtype=torch.int8, device=device)
+    buf = torch.empty(M, kp, dtype=_I8, device=device)
     return (buf if kp == K else buf[:, :K]), kp
 
 
@@ -87,12 +97,28 @@ def _padded_codes(q: torch.Tensor) -> torch.Tensor:
     return q if K % 16 == 0 else torch.nn.functional.pad(q, (0, -K % 16))[:, :K]
 
 
-def _launch(name: str, args, t: torch.Tensor) -> None:
-    if t.device.index == torch.cuda.current_device():
-        H.launch(name, args)
-    else:
-        with torch.cuda.device(t.device):
-            H.launch(name, args)
+def _vector(device: torch.device, what: str, s: torch.Tensor, shape) -> torch.Tensor:
+    """Scales or biases of ``shape`` as contiguous fp32 (their shape may stay that of several dimensions)."""
+    if s.shape != shape:
+        raise ValueError(f"{what} has shape {tuple(s.shape)}, expected {tuple(shape)}")
+    if s.device != device:
+        raise ValueError(f"{what} is on {s.device}, not on {device}")
+    if s.dtype is not _F32:
+        if not s.is_floating_point():
+            raise TypeError(f"{what} must be a floating tensor, not {s.dtype}")
+        s = s.float()
+    return s if s.is_contiguous() else s.contiguous()
+
+
+def _codes_given(q: torch.Tensor, what: str) -> None:
+    if q.dtype is not _I8:
+        raise TypeError(f"{what} must be int8, not {q.dtype}")
+
+
+def _launch(name: str, args, device: torch.device) -> None:
+    rc = H.launch_on(name, args, device.index)
+    if rc:
+        H._check(rc, name)
 
 
 def _shaped(t: torch.Tensor, x: torch.Tensor, *last: int) -> torch.Tensor:
@@ -100,57 +126,42 @@ def _shaped(t: torch.Tensor, x: torch.Tensor, *last: int) -> torch.Tensor:
     return t if x.ndim == 2 else t.view((*x.shape[:-1], *last))
 
 
-@torch.no_grad()
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """``x[..., K]`` (fp32 / bf16 / fp16) -> ``(codes[..., K] int8, scale[...] fp32)``:
     ``scale = max |row| / 127``, ``code = round(x * 127 / max |row|)``, halves to even."""
     dt = _float_code(x, "x")
-    x2, M, K = _rows(x, "x")
+    x2 = _rows(x, "x")
+    M, K = x2.shape
     if not x.is_cuda:
-        q, scale = ref.quantize_rows(x2)
-        return _shaped(_padded_codes(q), x, K), _shaped(scale, x)
-    q, ld = _new_codes(M, K, x.device)
-    scale = torch.empty(M, dtype=torch.float32, device=x.device)
+        with torch.no_grad():
+            q, scale = ref.quantize_rows(x2)
+            return _shaped(_padded_codes(q), x, K), _shaped(scale, x)
+    device = x.device
+    q, ld = _new_codes(M, K, device)
+    scale = torch.empty(M, dtype=_F32, device=device)
     if M:
-        a = H.QuantRowsArgs()
-        a.x, a.q, a.scale = x2.data_ptr(), q.data_ptr(), scale.data_ptr()
-        a.M, a.K, a.ld_x, a.ld_q = M, K, x2.stride(0), ld
-        a.dtype, a.wdtype = dt, H.F_NONE
-        _launch("d4pg_quant_rows", a, x)
-    return _shaped(q, x, K), _shaped(scale, x)
+        _launch("d4pg_quant_rows", H.QuantRowsArgs(x2.data_ptr(), None, None, None, q.data_ptr(), scale.data_ptr(), M, K,
+                                                   x2.stride(0), 0, 0, ld, dt, H.F_NONE, 0, 0.0), device)
+    return (q, scale) if x.ndim == 2 else (_shaped(q, x, K), _shaped(scale, x))
 
 
-@torch.no_grad()
 def dequantize_rows(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """``codes[..., K]``, ``scale[...]`` -> ``codes * scale`` in ``dtype``."""
     dt = _out_code(dtype)
-    if q.dtype != torch.int8:
-        raise TypeError(f"q must be int8, not {q.dtype}")
-    q2, M, K = _rows(q, "q")
-    s = _scales(q, "scale", scale, q.shape[:-1])
+    _codes_given(q, "q")
+    device = q.device
+    q2 = _rows(q, "q")
+    M, K = q2.shape
+    s = _vector(device, "scale", scale, q.shape[:-1])
     if not q.is_cuda:
-        return _shaped(ref.dequantize_rows(q2, s, dtype), q, K)
-    out = torch.empty(M, K, dtype=dtype, device=q.device)
+        with torch.no_grad():
+            return _shaped(ref.dequantize_rows(q2, s.reshape(-1), dtype), q, K)
+    out = torch.empty(M, K, dtype=dtype, device=device)
     if M:
-        a = H.DequantRowsArgs()
-        a.q, a.scale, a.out = q2.data_ptr(), s.data_ptr(), out.data_ptr()
-        a.M, a.K, a.ld_q, a.dtype = M, K, q2.stride(0), dt
-        _launch("d4pg_dequant_rows", a, q)
-    return _shaped(out, q, K)
+        _launch("d4pg_dequant_rows", H.DequantRowsArgs(q2.data_ptr(), s.data_ptr(), out.data_ptr(), M, K, q2.stride(0), dt, 0), device)
+    return out if q.ndim == 2 else _shaped(out, q, K)
 
 
-def _scales(near: torch.Tensor, what: str, s: torch.Tensor, shape) -> torch.Tensor:
-    if s.shape != shape:
-        raise ValueError(f"{what} has shape {tuple(s.shape)}, expected {tuple(shape)}")
-    _same_device(near, what, s)
-    if s.dtype != torch.float32:
-        if not s.is_floating_point():
-            raise TypeError(f"{what} must be a floating tensor, not {s.dtype}")
-        s = s.float()
-    return s if s.is_contiguous() and s.ndim == 1 else s.reshape(-1).contiguous()
-
-
-@torch.no_grad()
 def add_rms_norm_int8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
                       eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``h = x + residual``; ``y = h * weight / sqrt(mean(h^2) + eps)``; returns ``(codes of y, scales of y, h)``.
@@ -162,54 +173,50 @@ def add_rms_norm_int8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, re
     eps = float(eps)
     if not 0.0 <= eps < float("inf"):
         raise ValueError(f"eps must be a finite number >= 0, not {eps}")
-    x2, M, K = _rows(x, "x")
-    r2 = None
+    device = x.device
+    x2 = _rows(x, "x")
+    M, K = x2.shape
+    r2, wt = None, H.F_NONE
     if residual is not None:
         if residual.shape != x.shape or residual.dtype != x.dtype:
             raise ValueError(f"residual is {tuple(residual.shape)} {residual.dtype}, x is {tuple(x.shape)} {x.dtype}")
-        _same_device(x, "residual", residual)
-        r2 = _rows(residual, "residual")[0]
-    wt = H.F_NONE
+        _on(device, "residual", residual)
+        r2 = _rows(residual, "residual")
     if weight is not None:
         if weight.shape != (K,):
             raise ValueError(f"weight has shape {tuple(weight.shape)}, expected ({K},)")
         wt = _float_code(weight, "weight")
-        _same_device(x, "weight", weight)
+        _on(device, "weight", weight)
         weight = weight.contiguous()
     if not x.is_cuda:
-        q, scale, h = ref.add_rms_norm_int8(x2, weight, r2, eps)
-        return _shaped(_padded_codes(q), x, K), _shaped(scale, x), (x if residual is None else _shaped(h, x, K))
-    q, ld = _new_codes(M, K, x.device)
-    scale = torch.empty(M, dtype=torch.float32, device=x.device)
-    h = None if r2 is None else torch.empty(M, K, dtype=x.dtype, device=x.device)
+        with torch.no_grad():
+            q, scale, h = ref.add_rms_norm_int8(x2, weight, r2, eps)
+            return _shaped(_padded_codes(q), x, K), _shaped(scale, x), (x if residual is None else _shaped(h, x, K))
+    q, ld = _new_codes(M, K, device)
+    scale = torch.empty(M, dtype=_F32, device=device)
+    h = x if r2 is None else torch.empty(M, K, dtype=x.dtype, device=device)
     if M:
-        a = H.QuantRowsArgs()
-        a.x, a.q, a.scale = x2.data_ptr(), q.data_ptr(), scale.data_ptr()
-        a.M, a.K, a.ld_x, a.ld_q = M, K, x2.stride(0), ld
-        a.dtype, a.wdtype, a.norm, a.eps = dt, wt, 1, eps
-        if weight is not None:
-            a.weight = weight.data_ptr()
-        if r2 is not None:
-            a.residual, a.ld_r, a.h, a.ld_h = r2.data_ptr(), r2.stride(0), h.data_ptr(), K
-        _launch("d4pg_quant_rows", a, x)
-    return _shaped(q, x, K), _shaped(scale, x), (x if h is None else _shaped(h, x, K))
+        _launch("d4pg_quant_rows", H.QuantRowsArgs(
+            x2.data_ptr(), None if r2 is None else r2.data_ptr(), None if weight is None else weight.data_ptr(),
+            None if r2 is None else h.data_ptr(), q.data_ptr(), scale.data_ptr(), M, K, x2.stride(0),
+            0 if r2 is None else r2.stride(0), K, ld, dt, wt, 1, eps), device)
+    if x.ndim == 2:
+        return q, scale, h
+    return _shaped(q, x, K), _shaped(scale, x), (x if r2 is None else _shaped(h, x, K))
 
 
-def _layer_checks(K: int, near: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
-                  bias: Optional[torch.Tensor]):
-    """``(weight scales, bias)`` as the kernels read them."""
-    if weight.dtype != torch.int8:
-        raise TypeError(f"weight must be int8, not {weight.dtype}")
+def _layer(device: torch.device, K: int, weight: torch.Tensor, weight_scale: torch.Tensor, bias: Optional[torch.Tensor]):
+    """``(weight scales, bias)`` of a layer with ``K`` inputs, as the kernels read them."""
+    _codes_given(weight, "weight")
     if weight.ndim != 2 or weight.shape[1] != K:
         raise ValueError(f"weight has shape {tuple(weight.shape)}, expected (out, {K})")
     if K > MAX_K:
         raise ValueError(f"{K} columns: sums of more than {MAX_K} products can leave 32 bits")
-    _same_device(near, "weight", weight)
-    ws = _scales(near, "weight_scale", weight_scale, weight.shape[:1])
-    return ws, None if bias is None else _scales(near, "bias", bias, weight.shape[:1])
+    _on(device, "weight", weight)
+    outs = weight.shape[:1]
+    return _vector(device, "weight_scale", weight_scale, outs), None if bias is None else _vector(device, "bias", bias, outs)
 
 
-@torch.no_grad()
 def linear_int8(q: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
                 bias: Optional[torch.Tensor] = None, activation: str = "none",
                 dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -218,46 +225,82 @@ def linear_int8(q: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, weig
     ``q[..., K]`` int8 with ``scale[...]``; ``weight[N, K]`` int8 with ``weight_scale[N]``; ``bias[N]`` or ``None``;
     ``activation`` in {none, relu, tanh}; ``dtype`` fp32, bf16 or fp16."""
     dt = _out_code(dtype)
-    if activation not in _ACTS:
-        raise ValueError(f"activation must be one of {sorted(_ACTS)}, not {activation!r}")
-    if q.dtype != torch.int8:
-        raise TypeError(f"q must be int8, not {q.dtype}")
+    act = _act_code(activation)
+    _codes_given(q, "q")
+    device = q.device
     if q.ndim < 1 or q.shape[-1] < 1:
         raise ValueError(f"q needs at least one column, not shape {tuple(q.shape)}")
-    ws, b = _layer_checks(q.shape[-1], q, weight, weight_scale, bias)
-    s = _scales(q, "scale", scale, q.shape[:-1])
+    K = q.shape[-1]
+    ws, b = _layer(device, K, weight, weight_scale, bias)
+    s = _vector(device, "scale", scale, q.shape[:-1])
     N = weight.shape[0]
     if not q.is_cuda:
-        y = ref.linear_int8(_rows(q, "q")[0], s, weight, ws, b, activation, dtype)
-        return _shaped(y, q, N)
-    q2, M, K, ldq = _code_rows(q, "q")
-    out = torch.empty(M, N, dtype=dtype, device=q.device)
+        with torch.no_grad():
+            return _shaped(ref.linear_int8(_rows(q, "q"), s.reshape(-1), weight, ws, b, activation, dtype), q, N)
+    q2, ldq = _code_rows(q, "q")
+    M = q2.shape[0]
+    out = torch.empty(M, N, dtype=dtype, device=device)
     if M and N:
-        w2, _, _, ldw = _code_rows(weight, "weight")
-        a = H.LinearInt8Args()
-        a.q, a.scale, a.w, a.wscale, a.out = q2.data_ptr(), s.data_ptr(), w2.data_ptr(), ws.data_ptr(), out.data_ptr()
-        if b is not None:
-            a.bias = b.data_ptr()
-        a.ld_q, a.ld_w, a.ld_out = ldq, ldw, N
-        a.M, a.N, a.K, a.act, a.dtype = M, N, K, _ACTS[activation], dt
-        _launch("d4pg_linear_int8", a, q)
-    return _shaped(out, q, N)
+        w2, ldw = _code_rows(weight, "weight")
+        _launch("d4pg_linear_int8", H.LinearInt8Args(
+            q2.data_ptr(), s.data_ptr(), w2.data_ptr(), ws.data_ptr(), None if b is None else b.data_ptr(), out.data_ptr(),
+            ldq, ldw, N, M, N, K, act, dt, 0), device)
+    return out if q.ndim == 2 else _shaped(out, q, N)
+
+
+_FINAL = ("none", "relu", "softmax", "tanh")
 
 
 def mlp3_int8(x: torch.Tensor, layers: Sequence[Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]],
               final: str = "none", dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """Three-layer MLP of the actor / critic on 8-bit codes (ReLU, ReLU, ``final`` in {none, relu, tanh, softmax}).
 
-    ``layers``: three ``(weight[out, in] int8, weight_scale[out], bias[out] or None)``.  The input of every layer is
-    quantised per row; what the layers hand on is fp32; the result is in ``dtype``."""
+    ``x[..., S]`` fp32, bf16 or fp16; ``layers``: three ``(weight[out, in] int8, weight_scale[out], bias[out] or None)``.
+    The input of every layer is quantised per row; what the layers hand on is fp32; the result is in ``dtype``.  On the GPU
+    the network is one launch (``mlp3_int8_kernel``) up to 2048 columns, and a launch per step beyond."""
+    dt = _out_code(dtype)
     if len(layers) != 3:
         raise ValueError(f"three layers are expected, not {len(layers)}")
-    _out_code(dtype)
-    if final not in ("none", "relu", "tanh", "softmax"):
-        raise ValueError(f"final must be none, relu, tanh or softmax, not {final!r}")
+    if final not in _FINAL:
+        raise ValueError(f"final must be one of {_FINAL}, not {final!r}")
+    if final == "softmax":
+        return torch.softmax(mlp3_int8(x, layers), dim=-1).to(dtype)
+    if x.is_cuda:
+        out = _mlp3_fused(x, layers, final, dtype, dt)
+        if out is not None:
+            return out
     h = x
     for weight, weight_scale, bias in layers[:2]:
         h = linear_int8(*quantize_rows(h), weight, weight_scale, bias, "relu")
-    if final == "softmax":
-        return torch.softmax(linear_int8(*quantize_rows(h), *layers[2]), dim=-1).to(dtype)
     return linear_int8(*quantize_rows(h), *layers[2], activation=final, dtype=dtype)
+
+
+def _mlp3_fused(x: torch.Tensor, layers, final: str, dtype: torch.dtype, dt: int) -> Optional[torch.Tensor]:
+    xdt = _float_code(x, "x")
+    x2 = _rows(x, "x")
+    device = x.device
+    M, K = x2.shape
+    a = H.Mlp3Int8Args()
+    held, width = [], [K]
+    for i, (weight, weight_scale, bias) in enumerate(layers):
+        ws, b = _layer(device, K, weight, weight_scale, bias)
+        K = weight.shape[0]
+        if K < 1:
+            return None
+        w2, a.ld_w[i] = _code_rows(weight, "weight")
+        a.w[i], a.wscale[i] = w2.data_ptr(), ws.data_ptr()
+        if b is not None:
+            a.bias[i] = b.data_ptr()
+        held.append((w2, ws, b))
+        width.append(K)
+    out = torch.empty(M, K, dtype=dtype, device=device)
+    if M:
+        a.width[:] = width
+        a.x, a.ld_x, a.out, a.ld_out, a.M = x2.data_ptr(), x2.stride(0), out.data_ptr(), K, M
+        a.xdtype, a.dtype, a.act = xdt, dt, _ACTS[final]
+        rc = H.launch_on("d4pg_mlp3_int8", a, device.index)
+        if rc == 1:              # too wide for one workgroup's LDS
+            return None
+        if rc:
+            H._check(rc, "d4pg_mlp3_int8")
+    return out if x.ndim == 2 else _shaped(out, x, K)

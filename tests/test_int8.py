@@ -402,6 +402,33 @@ def test_mlp3_int8(B, S, H, A, final, device):
     assert ops.mlp3_int8(x.reshape(1, B, S), layers, final, torch.bfloat16).shape == (1, B, A)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,dims", [(1, (24, 400, 400, 4)), (5, (3, 64, 64, 1)), (17, (111, 128, 130, 51)), (33, (8, 256, 256, 2)), (40, (376, 300, 77, 300)),
+                                    (2049, (17, 400, 400, 6)), (2100, (111, 1024, 1024, 8)), (31, (2048, 40, 2048, 2048)), (2200, (9, 2000, 1500, 33)),
+                                    (3, (5, 2100, 2100, 3)), (4, (2500, 64, 64, 2)), (1, (1, 1, 1, 1)), (9, (63, 65, 16, 17)), (16, (64, 144, 129, 128))])
+def test_mlp3_int8_is_the_layers_one_by_one(B, dims):
+    """One launch or seven: the same values to the last bit, for every way columns and rows are dealt out."""
+    x = _randn(B, dims[0], seed=B).cuda()
+    x[0] = 0.0
+    if B > 2:
+        x[1, dims[0] // 2] = math.nan
+    layers = _layers([(dims[i + 1], dims[i]) for i in range(3)], "cuda", seed=B, bias=B % 2 == 0)
+    for final, dtype, xt in (("tanh", torch.float32, torch.float32), ("none", torch.bfloat16, torch.bfloat16), ("relu", torch.float16, torch.float16)):
+        h = x.to(xt)
+        want = h
+        for i, (w, ws, b) in enumerate(layers):
+            want = ops.linear_int8(*ops.quantize_rows(want), w, ws, b, "relu" if i < 2 else final, torch.float32 if i < 2 else dtype)
+        got = ops.mlp3_int8(h, layers, final, dtype)
+        assert got.dtype == dtype and torch.equal(torch.isnan(got), torch.isnan(want))
+        assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))
+        assert B <= 2 or torch.isnan(got[1]).all()
+    strided = torch.zeros(B, 2 * dims[0] + 3, device="cuda")
+    strided[:, 1:1 + 2 * dims[0]:2] = x
+    view = strided[:, 1:1 + dims[0]]
+    want = ops.mlp3_int8(view.contiguous(), layers)
+    assert torch.equal(torch.nan_to_num(ops.mlp3_int8(view, layers)), torch.nan_to_num(want))
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_a_residual_block_of_them(device):
     """norm -> product -> norm of the sum -> product, as a residual network calls them, against fp64 layers without any
