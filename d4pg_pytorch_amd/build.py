@@ -6,6 +6,8 @@
   device pointers are shared with torch.
 * ``csrc/libd4pg_host.so`` — C++ host runtime (shared-memory transition rings,
   seq-locked weight slab, n-step assembler, OU noise, CPU actor inference), ``g++``.
+* ``csrc/_d4pg_int8.so``   — tensor binding of the 8-bit operators (a Python extension module), ``g++`` against the
+  headers of the installed torch.
 
 Run ``python -m d4pg_pytorch_amd.build`` or call :func:`build_all`.
 """
@@ -24,7 +26,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 HIP_SOURCES = ["gemm.hip", "loss.hip", "optim.hip", "replay.hip", "nstep.hip", "fused.hip", "fused32.hip", "rollout.hip", "int8.hip", "planar_env.hip", "analytic_env.hip", "ant_env.hip"]
 HOST_SOURCES = ["host_runtime.cpp", "planar_host.cpp"]
+BIND_SOURCES = ["int8_bind.cpp"]
 HIP_LIB = os.path.join(CSRC, "libd4pg_hip.so")
+BIND_LIB = os.path.join(CSRC, "_d4pg_int8.so")
 HOST_LIB = os.path.join(CSRC, "libd4pg_host.so")
 ARCH = "gfx950"
 
@@ -191,13 +195,40 @@ def build_host(force: bool = False, verbose: bool = False) -> str:
     return HOST_LIB
 
 
+def build_bind(force: bool = False, verbose: bool = False) -> str:
+    import sysconfig
+    import torch
+    inc, tl = os.path.join(os.path.dirname(torch.__file__), "include"), torch_lib_dir()
+    srcs = [os.path.join(CSRC, s) for s in BIND_SOURCES]
+    tmp = BIND_LIB + ".tmp"
+    cmd = ["g++", "-O2", "-fPIC", "-shared", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-isystem", inc,
+           "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"),
+           "-isystem", os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_hipcc()))), "include"),
+           "-isystem", sysconfig.get_paths()["include"]] + srcs + \
+          ["-o", tmp, f"-L{tl}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip", "-l:libamdhip64.so"]
+    # the module holds torch's class layouts: another torch is another build
+    digest = _digest(cmd + [torch.__version__], sorted({f for s in srcs for f in _closure(s)}))
+    if not force and _recorded(BIND_LIB) == digest:
+        LAST_BUILD["bind"] = "reused (digest of sources, flags and torch matches the library's manifest)"
+        return BIND_LIB
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    _run(cmd)
+    os.replace(tmp, BIND_LIB)
+    _record(BIND_LIB, digest, {})
+    LAST_BUILD["bind"] = f"compiled {len(srcs)} sources, linked"
+    return BIND_LIB
+
+
 def build_all(force: bool = False, verbose: bool = False) -> None:
     build_host(force, verbose)
     build_hip(force, verbose)
+    build_bind(force, verbose)
     if verbose:
-        print(f"build: host runtime {LAST_BUILD['host']}; HIP kernels {LAST_BUILD['hip']}", flush=True)
+        print(f"build: host runtime {LAST_BUILD['host']}; HIP kernels {LAST_BUILD['hip']}; tensor binding {LAST_BUILD['bind']}", flush=True)
 
 
 if __name__ == "__main__":
     build_all(force="--force" in sys.argv, verbose=True)
-    print("built:", HIP_LIB, HOST_LIB)
+    print("built:", HIP_LIB, HOST_LIB, BIND_LIB)

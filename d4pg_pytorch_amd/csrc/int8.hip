@@ -14,10 +14,9 @@
 //  * A row that holds a NaN or an infinity gets scale NaN and codes 0: whatever reads it gets NaN, never a number.
 //  * A row of zeros gets scale 0 and codes 0.
 #include "common.h"
+#include "int8_args.h"
 #include <type_traits>
 
-enum { F_FP32 = 0, F_BF16 = 1, F_FP16 = 2, F_NONE = -1 };
-enum { ACT_NONE = 0, ACT_RELU = 1, ACT_TANH = 2 };
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
@@ -25,19 +24,6 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 // ---------------------------------------------------------------------------------------------------------------
 // floating rows -> codes
 // ---------------------------------------------------------------------------------------------------------------
-struct QuantRowsArgs {
-    const void* x;         // [M, K] rows of ld_x elements
-    const void* residual;  // [M, K] added to x, or null                       (norm only)
-    const void* weight;    // [K] factor after the norm, or null               (norm only)
-    void* h;               // [M, K] x + residual in x's type, or null         (norm only)
-    signed char* q;        // [M, ld_q] codes, zero from K to ld_q
-    float* scale;          // [M]
-    long long M, K;
-    long long ld_x, ld_r, ld_h, ld_q;   // elements (bytes for ld_q, a multiple of 16)
-    int dtype, wdtype;     // F_*: of x, residual and h; of weight
-    int norm;              // 0: quantise x; 1: RMS norm first
-    float eps;
-};
 
 // Eight neighbouring elements of a row.  Only the element's own alignment is assumed: gfx950 takes 16-byte loads and
 // stores at any address, so rows of odd length need no path of their own (the last K % 8 elements aside).
@@ -375,13 +361,6 @@ D4PG_API int d4pg_quant_rows(const QuantRowsArgs* a, hipStream_t stream) {
 // ---------------------------------------------------------------------------------------------------------------
 // codes -> floating rows
 // ---------------------------------------------------------------------------------------------------------------
-struct DequantRowsArgs {
-    const signed char* q;  // [M, K] rows of ld_q bytes
-    const float* scale;    // [M]
-    void* out;             // [M, K] contiguous
-    long long M, K, ld_q;
-    int dtype, tpr_log;    // threads a row = 2^tpr_log (set by the host entry)
-};
 
 template <typename T>
 __global__ __launch_bounds__(256) void dequant_rows_kernel(const DequantRowsArgs a) {
@@ -421,17 +400,6 @@ D4PG_API int d4pg_dequant_rows(DequantRowsArgs* a, hipStream_t stream) {
 // ---------------------------------------------------------------------------------------------------------------
 // product of codes
 // ---------------------------------------------------------------------------------------------------------------
-struct LinearInt8Args {
-    const signed char* q;  // [M, K] activations' codes, rows of ld_q bytes
-    const float* scale;    // [M]
-    const signed char* w;  // [N, K] weights' codes, rows of ld_w bytes
-    const float* wscale;   // [N]
-    const float* bias;     // [N] or null
-    void* out;             // [M, N], rows of ld_out elements
-    long long ld_q, ld_w, ld_out;
-    int M, N, K;
-    int act, dtype, pad_;
-};
 
 __device__ __forceinline__ float act_of(float y, int act) {
     if (act == ACT_RELU) return y < 0.f ? 0.f : y;        // keeps NaN
@@ -756,18 +724,6 @@ D4PG_API int d4pg_linear_int8(const LinearInt8Args* a, hipStream_t stream) {
 // A layer whose columns make more than 8 tiles of 16 deals them to the waves (TPW each); a narrower one deals K, the waves
 // of a tile meeting in LDS integer additions.  Codes lie in LDS in rows 16 bytes apart from a multiple of 64, zero from the
 // layer's width up to it: the 16 lanes of an LDS cycle cover all banks, and what the weights hold beyond K meets zeros.
-struct Mlp3Int8Args {
-    const void* x;                 // [M, width[0]] rows of ld_x elements
-    void* out;                     // [M, width[3]] rows of ld_out elements
-    const signed char* w[3];       // [width[i + 1], width[i]] codes, rows of ld_w[i] bytes
-    const float* wscale[3];
-    const float* bias[3];          // or null
-    long long ld_x, ld_out, ld_w[3];
-    int M, width[4];
-    int xdtype, dtype, act;        // F_* of x and out; ACT_* of the last layer (the others: ReLU)
-    int pad_;
-    int pitch, split;              // bytes of a row of codes in LDS, words of the split layers' sums (set by the host entry)
-};
 constexpr int MLP_WAVES = 16;
 
 __device__ __forceinline__ float load_any(const void* p, int dtype, long long i) {
@@ -776,34 +732,62 @@ __device__ __forceinline__ float load_any(const void* p, int dtype, long long i)
     return load1<_Float16>(p, i);
 }
 
-// The products of NT column tiles n0[j] .. n0[j] + 15 with the workgroup's rows, over slices of 64 k from k0 on, `step`
-// apart.  The loads of U slices are issued before the first product.
-template <int NT, int MT, int U>
-__device__ __forceinline__ void mlp_product(i32x4 (&acc)[NT][MT], const signed char* w, long long ld, int N, int K, const int (&n0)[NT],
-                                            const signed char* codes, int pitch, int k0, int step) {
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, last = ((K - 1) >> 4) << 4;
-    const signed char* wp[NT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) wp[j] = w + (long long)min(n0[j] + c, N - 1) * ld;
-    const signed char* const xp = codes + c * pitch + 16 * g;
-    for (int k = k0; k < K; k += step * U) {
-        i32x4 wf[U][NT];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) wf[u][j] = *reinterpret_cast<const i32x4*>(wp[j] + min(k + u * step + 16 * g, last));
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (k + u * step >= K) break;        // the same for the wave
-            i32x4 xf[MT];
-#pragma unroll
-            for (int i = 0; i < MT; ++i) xf[i] = *reinterpret_cast<const i32x4*>(xp + i * 16 * pitch + k + u * step);
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int i = 0; i < MT; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u][j], xf[i], acc[j][i], 0, 0, 0);
-        }
+// The wave's weights, layer after layer, as one stream of units: 16 rows x 64 k (1 KB), moved from memory into the wave's
+// own ring in LDS (no registers, no barrier).  RING - 1 units are on their way ahead of the one that is multiplied, across
+// the borders of slices and layers: weights depend on nothing.  An instruction moves 16 rows of 64 neighbouring bytes in
+// lane order; read straight into the matrix operand's order, lane 16 g + c row c, the same bytes cost five times as much
+// (16 rows behind every 16 lanes: 41 us for a network of 1024 columns instead of @).
+// 16-byte pieces of a row lie XOR (row / 4): the 16 lanes of an LDS cycle then cover all banks.
+__device__ __forceinline__ void lds_barrier() {          // LDS is settled for the workgroup; moves stay on their way
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+struct MlpStream {
+    int layer, slice, j;           // of the next unit to move
+    int moved, used;               // ring slots
+};
+// How a layer's units are dealt: a wave has `count` tiles tile0, tile0 + 16, ... and slices of 64 k from k0 on, `step` apart.
+struct MlpShare {
+    int K, N, tiles, count, tile0, k0, step, slices;
+    bool narrow;
+};
+__device__ __forceinline__ MlpShare mlp_share(const Mlp3Int8Args& a, int layer, int wave) {
+    MlpShare s;
+    s.K = a.width[layer], s.N = a.width[layer + 1], s.tiles = (s.N + 15) >> 4;
+    s.narrow = s.tiles <= MLP_WAVES / 2;
+    const int spread = !s.narrow ? MLP_WAVES : s.tiles <= 1 ? 1 : (s.tiles <= 2 ? 2 : (s.tiles <= 4 ? 4 : 8));
+    const int parts = MLP_WAVES / spread, part = wave / spread;
+    s.tile0 = wave & (spread - 1);
+    s.count = s.tile0 < s.tiles ? (s.narrow ? 1 : (s.tiles - s.tile0 + MLP_WAVES - 1) / MLP_WAVES) : 0;
+    s.k0 = 64 * part, s.step = 64 * parts;
+    s.slices = s.count ? (s.K - s.k0 + s.step - 1) / s.step : 0;
+    if (s.slices < 0) s.slices = 0;
+    return s;
+}
+template <int RING>
+__device__ __forceinline__ bool mlp_move(const Mlp3Int8Args& a, MlpStream& st, MlpShare& s, signed char* ring, int wave, int lane) {
+    while (st.layer < 3 && st.slice >= s.slices) {       // the next layer that has anything for this wave
+        ++st.layer, st.slice = 0, st.j = 0;
+        if (st.layer < 3) s = mlp_share(a, st.layer, wave);
     }
+    if (st.layer >= 3) return false;
+    const int row = lane >> 2, piece = (lane & 3) ^ (lane >> 4);
+    const int n = min(16 * (s.tile0 + MLP_WAVES * st.j) + row, s.N - 1);
+    const int k = min(s.k0 + st.slice * s.step + 16 * piece, ((s.K - 1) >> 4) << 4);
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(a.w[st.layer] + (long long)n * a.ld_w[st.layer] + k),
+                                     (__attribute__((address_space(3))) void*)(ring + st.moved * 1024), 16, 0, 0);
+    st.moved = st.moved + 1 == RING ? 0 : st.moved + 1;
+    if (++st.j == s.count) st.j = 0, ++st.slice;
+    return true;
+}
+// Moves one more unit and returns the next one's place in LDS once it has arrived.
+template <int RING>
+__device__ __forceinline__ const signed char* mlp_next(const Mlp3Int8Args& a, MlpStream& st, MlpShare& ahead, signed char* ring, int wave, int lane) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the slot that is moved into has been read
+    if (mlp_move<RING>(a, st, ahead, ring, wave, lane)) asm volatile("s_waitcnt vmcnt(%0)" :: "n"(RING - 1) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const signed char* const unit = ring + st.used * 1024;
+    st.used = st.used + 1 == RING ? 0 : st.used + 1;
+    return unit;
 }
 
 // Codes of row r, columns n .. n + 3 of one lane's values.
@@ -815,133 +799,142 @@ __device__ __forceinline__ void mlp_codes(signed char* codes, int pitch, int r, 
 }
 
 template <int TPW, int MT>
-__global__ __launch_bounds__(64 * MLP_WAVES) void mlp3_int8_kernel(const Mlp3Int8Args a) {
-    extern __shared__ __attribute__((aligned(128))) signed char mem[];
-    constexpr int ROWS = 16 * MT, U = TPW * MT >= 16 ? 1 : (TPW * MT >= 8 ? 2 : 4);
+__device__ __forceinline__ void mlp3_rows(const Mlp3Int8Args& a, signed char* const mem) {
+    constexpr int ROWS = 16 * MT, RING = MT == 1 ? 8 : 6;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     const int m0 = blockIdx.x * ROWS, pitch = a.pitch;
-    signed char* const codes[2] = {mem, mem + ROWS * pitch};
-    int* const sums = reinterpret_cast<int*>(mem + 2 * ROWS * pitch);
+    signed char* const ring = mem + wave * RING * 1024;
+    signed char* const codes = mem + MLP_WAVES * RING * 1024;
+    int* const sums = reinterpret_cast<int*>(codes + ROWS * pitch);
     unsigned* const top = reinterpret_cast<unsigned*>(sums + a.split);       // [3][ROWS] largest magnitudes, as bits
 
+    MlpShare ahead = mlp_share(a, 0, wave);
+    MlpStream st = {0, 0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < RING - 1; ++i) mlp_move<RING>(a, st, ahead, ring, wave, lane);
+
     for (int i = threadIdx.x; i < a.split; i += 64 * MLP_WAVES) sums[i] = 0;
-    for (int i = threadIdx.x; i < 3 * ROWS; i += 64 * MLP_WAVES) top[i] = 0u;
-    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * ROWS; i += 64 * MLP_WAVES) top[ROWS + i] = 0u;
     {
         const int S = a.width[0], padded = (S + 63) & ~63;
         for (int r = wave; r < ROWS; r += MLP_WAVES) {
             const long long row = (long long)min(m0 + r, a.M - 1) * a.ld_x;
+            constexpr int HELD = 4;              // 64-element pieces of a row kept from the first pass to the second
+            float held[HELD];
             unsigned t = 0;
-            for (int k = lane; k < S; k += 64) t = max(t, abs_bits(load_any(a.x, a.xdtype, row + k)));
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) {
+                const int k = lane + 64 * i;
+                held[i] = load_any(a.x, a.xdtype, row + min(k, S - 1));
+                t = max(t, abs_bits(held[i]));   // beyond S: the last element again
+            }
+            for (int k = lane + 64 * HELD; k < S; k += 64) t = max(t, abs_bits(load_any(a.x, a.xdtype, row + k)));
             t = wave_umax(t);
             if (lane == 0) top[r] = t;
             const RowCode rc = row_code(t);
-            for (int k = lane; k < padded; k += 64)
-                codes[0][r * pitch + k] = k < S ? (signed char)(code_bits(load_any(a.x, a.xdtype, row + k), rc) & rc.keep) : 0;
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) {
+                const int k = lane + 64 * i;
+                if (k < padded) codes[r * pitch + k] = k < S ? (signed char)(code_bits(held[i], rc) & rc.keep) : 0;
+            }
+            for (int k = lane + 64 * HELD; k < padded; k += 64)
+                codes[r * pitch + k] = k < S ? (signed char)(code_bits(load_any(a.x, a.xdtype, row + k), rc) & rc.keep) : 0;
         }
     }
-    __syncthreads();
+    lds_barrier();
+    const signed char* const xp = codes + c * pitch + 16 * g;
+    const int wo = c * 64 + (g ^ (c >> 2)) * 16; // this lane's piece of a unit
     for (int layer = 0; layer < 3; ++layer) {
-        const int K = a.width[layer], N = a.width[layer + 1], tiles = (N + 15) >> 4;
-        const signed char* const w = a.w[layer];
+        const MlpShare s = mlp_share(a, layer, wave);
+        const int N = s.N;
         const float* const wscale = a.wscale[layer];
         const float* const bias = a.bias[layer];
-        const signed char* const in = codes[layer & 1];
-        signed char* const next = codes[(layer & 1) ^ 1];
         const int act = layer < 2 ? ACT_RELU : a.act;
         const unsigned* const top_in = top + layer * ROWS;
-        // zeros from the layer's width up to the next slice (whole tiles write their own)
-        if (layer < 2)
-            for (int i = threadIdx.x; i < ROWS * 4; i += 64 * MLP_WAVES) {
-                const int n = (N & ~63) + 16 * (i & 3);
-                if ((N & 63) && n >= 16 * tiles) *reinterpret_cast<i32x4*>(next + (i >> 2) * pitch + n) = i32x4{0, 0, 0, 0};
+        unsigned* const top_out = top + (layer + 1) * ROWS;
+        i32x4 acc[TPW][MT] = {};
+        for (int sl = 0; sl < s.slices; ++sl) {
+            i32x4 xf[MT];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) xf[i] = *reinterpret_cast<const i32x4*>(xp + i * 16 * pitch + s.k0 + sl * s.step);
+#pragma unroll
+            for (int j = 0; j < TPW; ++j) {
+                if (j >= s.count) break;
+                const i32x4 wf = *reinterpret_cast<const i32x4*>(mlp_next<RING>(a, st, ahead, ring, wave, lane) + wo);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf, xf[i], acc[j][i], 0, 0, 0);
             }
-        if (tiles <= MLP_WAVES / 2) {
-            // few columns: the waves of a tile share K
-            const int lanes_of_tiles = tiles <= 1 ? 1 : (tiles <= 2 ? 2 : (tiles <= 4 ? 4 : 8)), parts = MLP_WAVES / lanes_of_tiles;
-            const int tile = wave & (lanes_of_tiles - 1), part = wave / lanes_of_tiles;
-            int* const sum = sums + (tile * MT * 64 + lane) * 4;
-            if (tile < tiles) {
-                i32x4 acc[1][MT] = {};
-                const int n0[1] = {tile * 16};
-                mlp_product<1, MT, 4>(acc, w, a.ld_w[layer], N, K, n0, in, pitch, 64 * part, 64 * parts);
+        }
+        // Values of this wave: wide layers TPW x MT tiles; narrow ones the sums of all waves, dealt out again as units
+        // (tile, 16 rows), of which a wave has at most MT / 2 rounded up.
+        float v[TPW][MT][4];
+        unsigned m[MT] = {};
+        auto finish = [&](float (&y)[4], const i32x4 sum, int r, int n, unsigned& most) {
+            values4(y, sum, row_code(top_in[r]).scale, columns4(wscale, bias, n, N), bias != nullptr, act);
+            if (layer == 2) {
+                if (m0 + r < a.M && n < N) store_values4(a.out, (long long)(m0 + r) * a.ld_out + n, a.dtype, y, N - n);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) most = max(most, n + e < N ? abs_bits(y[e]) : 0u);
+            }
+        };
+        const int unit = wave, ut = unit / MT, ui = unit % MT;
+        if (s.narrow) {
+            if (s.count) {
+                int* const sum = sums + (s.tile0 * MT * 64 + lane) * 4;
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) atomicAdd(sum + i * 256 + e, acc[0][i][e]);
             }
-            __syncthreads();
-            // units (tile, i): at most 8 MT of them, MT / 2 a wave
-            float v[(MT + 1) / 2][4];
-#pragma unroll
-            for (int u = 0; u < (MT + 1) / 2; ++u) {
-                const int unit = wave + u * MLP_WAVES, t = unit / MT, i = unit % MT, n = 16 * t + 4 * g, r = 16 * i + c;
-                if (t >= tiles) continue;
-                int* const from = sums + (unit * 64 + lane) * 4;
-                const i32x4 s = *reinterpret_cast<const i32x4*>(from);
-                *reinterpret_cast<i32x4*>(from) = i32x4{0, 0, 0, 0};           // for the next layer that needs them
-                values4(v[u], s, row_code(top_in[r]).scale, columns4(wscale, bias, n, N), bias != nullptr, act);
-                if (layer == 2) {
-                    if (m0 + r < a.M && n < N) store_values4(a.out, (long long)(m0 + r) * a.ld_out + n, a.dtype, v[u], N - n);
-                } else {
-                    unsigned m = 0;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) m = max(m, n + e < N ? abs_bits(v[u][e]) : 0u);
-                    atomicMax(top + (layer + 1) * ROWS + r, m);
-                }
-            }
-            if (layer < 2) {
-                __syncthreads();
-#pragma unroll
-                for (int u = 0; u < (MT + 1) / 2; ++u) {
-                    const int unit = wave + u * MLP_WAVES, t = unit / MT, i = unit % MT, n = 16 * t + 4 * g, r = 16 * i + c;
-                    if (t < tiles) mlp_codes(next, pitch, r, n, N, v[u], row_code(top[(layer + 1) * ROWS + r]));
-                }
+            lds_barrier();
+            if (ut < s.tiles) {
+                i32x4* const from = reinterpret_cast<i32x4*>(sums + (unit * 64 + lane) * 4);
+                const i32x4 sum = *from;
+                *from = i32x4{0, 0, 0, 0};       // for the next layer that needs them
+                finish(v[0][0], sum, 16 * ui + c, 16 * ut + 4 * g, m[0]);
             }
         } else {
-            i32x4 acc[TPW][MT] = {};
-            int n0[TPW];
 #pragma unroll
-            for (int j = 0; j < TPW; ++j) n0[j] = 16 * (wave + j * MLP_WAVES);
-            mlp_product<TPW, MT, U>(acc, w, a.ld_w[layer], N, K, n0, in, pitch, 0, 64);
-            float v[TPW][MT][4];
-            unsigned m[MT] = {};
+            for (int j = 0; j < TPW; ++j)
+                if (j < s.count)
 #pragma unroll
-            for (int j = 0; j < TPW; ++j) {
-                const int n = n0[j] + 4 * g;
-                const Columns4 col = columns4(wscale, bias, n, N);
+                    for (int i = 0; i < MT; ++i) finish(v[j][i], acc[j][i], 16 * i + c, 16 * (s.tile0 + MLP_WAVES * j) + 4 * g, m[i]);
+        }
+        if (layer == 2) break;
 #pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    const int r = 16 * i + c;
-                    values4(v[j][i], acc[j][i], row_code(top_in[r]).scale, col, bias != nullptr, act);
-                    if (layer == 2) {
-                        if (m0 + r < a.M && n < N) store_values4(a.out, (long long)(m0 + r) * a.ld_out + n, a.dtype, v[j][i], N - n);
-                    } else {
+        for (int i = 0; i < MT; ++i) {
+            if (s.narrow && i > 0) break;
+            unsigned t = m[i];
+            t = max(t, (unsigned)__shfl_xor((int)t, 16, 64));
+            t = max(t, (unsigned)__shfl_xor((int)t, 32, 64));
+            if (g == 0) atomicMax(top_out + 16 * (s.narrow ? ui : i) + c, t);
+        }
+        lds_barrier();            // every wave has read the codes of this layer and given its largest
+        // zeros from the layer's width up to the next slice (whole tiles write their own)
+        if ((N & 63) && threadIdx.x < ROWS * 4) {
+            const int n = (N & ~63) + 16 * (threadIdx.x & 3);
+            if (n >= 16 * s.tiles) *reinterpret_cast<i32x4*>(codes + (threadIdx.x >> 2) * pitch + n) = i32x4{0, 0, 0, 0};
+        }
+        if (s.narrow) {
+            if (ut < s.tiles) mlp_codes(codes, pitch, 16 * ui + c, 16 * ut + 4 * g, N, v[0][0], row_code(top_out[16 * ui + c]));
+        } else {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) m[i] = max(m[i], n + e < N ? abs_bits(v[j][i][e]) : 0u);
-                    }
-                }
-            }
-            if (layer < 2) {
+            for (int i = 0; i < MT; ++i) {
+                const RowCode rc = row_code(top_out[16 * i + c]);
 #pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    unsigned t = m[i];
-                    t = max(t, (unsigned)__shfl_xor((int)t, 16, 64));
-                    t = max(t, (unsigned)__shfl_xor((int)t, 32, 64));
-                    if (g == 0) atomicMax(top + (layer + 1) * ROWS + 16 * i + c, t);
-                }
-                __syncthreads();
-#pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    const RowCode rc = row_code(top[(layer + 1) * ROWS + 16 * i + c]);
-#pragma unroll
-                    for (int j = 0; j < TPW; ++j)
-                        if (n0[j] < N) mlp_codes(next, pitch, 16 * i + c, n0[j] + 4 * g, N, v[j][i], rc);
-                }
+                for (int j = 0; j < TPW; ++j)
+                    if (j < s.count) mlp_codes(codes, pitch, 16 * i + c, 16 * (s.tile0 + MLP_WAVES * j) + 4 * g, N, v[j][i], rc);
             }
         }
-        __syncthreads();
+        lds_barrier();
     }
+}
+
+template <int TPW, int MT>
+__global__ __launch_bounds__(64 * MLP_WAVES) void mlp3_int8_kernel(const Mlp3Int8Args a) {
+    extern __shared__ __attribute__((aligned(128))) signed char net[];
+    mlp3_rows<TPW, MT>(a, net);
 }
 
 template <int TPW, int MT>
@@ -972,18 +965,20 @@ D4PG_API int d4pg_mlp3_int8(Mlp3Int8Args* a, hipStream_t stream) {
         if (tiles > wide_out) wide_out = tiles;
         if (tiles <= MLP_WAVES / 2 && tiles > few) few = tiles;
     }
-    if (widest > 2048 || wide_out > 128) return 1;
+    if (widest > 2048 || wide_out > 64) return 1;
     a->pitch = ((widest + 63) & ~63) + 16;
     int mt = a->pad_;
     if (mt == 0) mt = a->M <= 2048 ? 1 : 2;
     for (;; mt /= 2) {
         a->split = few * mt * 256;
-        const int lds = 2 * 16 * mt * a->pitch + 4 * a->split + 3 * 16 * mt * 4;
-        if (lds > 160 * 1024) continue;
+        const int lds = MLP_WAVES * (mt == 1 ? 8 : 6) * 1024 + 16 * mt * a->pitch + 4 * a->split + 3 * 16 * mt * 4;
+        if (lds > 160 * 1024) {
+            if (mt == 1) return 1;
+            continue;
+        }
         if (wide_out <= 16) return launch_mlp3_rows<1>(*a, mt, lds, stream);
         if (wide_out <= 32) return launch_mlp3_rows<2>(*a, mt, lds, stream);
-        if (wide_out <= 64) return launch_mlp3_rows<4>(*a, mt, lds, stream);
-        return launch_mlp3_rows<8>(*a, mt, lds, stream);
+        return launch_mlp3_rows<4>(*a, mt, lds, stream);
     }
 }
 

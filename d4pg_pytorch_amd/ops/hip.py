@@ -526,6 +526,28 @@ def lib() -> C.CDLL:
     return _lib
 
 
+_int8 = None
+
+
+def int8_binding():
+    """The tensor binding of the 8-bit operators (``csrc/int8_bind.cpp``), bound to the entries of :func:`lib`."""
+    global _int8
+    if _int8 is None:
+        import importlib.machinery
+        import importlib.util
+        path = os.path.join(os.path.dirname(_HERE), "csrc", "_d4pg_int8.so")
+        if not os.path.exists(path):
+            raise HipLibraryMissing(f"{path} not found: run `python -m d4pg_pytorch_amd.build`")
+        handle = lib()
+        loader = importlib.machinery.ExtensionFileLoader("_d4pg_int8", path)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_d4pg_int8", loader))
+        loader.exec_module(module)
+        module.bind(*(C.cast(getattr(handle, name), vp).value
+                      for name in ("d4pg_quant_rows", "d4pg_dequant_rows", "d4pg_linear_int8", "d4pg_mlp3_int8")))
+        _int8 = module
+    return _int8
+
+
 def _check(rc: int, what: str) -> None:
     if rc != 0:
         raise RuntimeError(f"{what} failed with code {rc}")

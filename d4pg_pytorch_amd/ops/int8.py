@@ -32,6 +32,18 @@ MAX_K = 131071
 _F32, _I8 = torch.float32, torch.int8
 
 
+#: the plain case of every operator in C++ (``csrc/int8_bind.cpp``; loaded with the first GPU tensor).  What it returns
+#: None for - other layouts, types and devices, mistakes - takes the way through the functions below.
+_plain = None
+
+
+def _binding():
+    global _plain
+    if _plain is None:
+        _plain = H.int8_binding()
+    return _plain
+
+
 def _float_code(t: torch.Tensor, what: str) -> int:
     code = _FLOATS.get(t.dtype)
     if code is None:
@@ -129,6 +141,10 @@ def _shaped(t: torch.Tensor, x: torch.Tensor, *last: int) -> torch.Tensor:
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """``x[..., K]`` (fp32 / bf16 / fp16) -> ``(codes[..., K] int8, scale[...] fp32)``:
     ``scale = max |row| / 127``, ``code = round(x * 127 / max |row|)``, halves to even."""
+    if x.is_cuda:
+        out = _binding().quantize(x)
+        if out is not None:
+            return out
     dt = _float_code(x, "x")
     x2 = _rows(x, "x")
     M, K = x2.shape
@@ -147,6 +163,10 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 
 def dequantize_rows(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """``codes[..., K]``, ``scale[...]`` -> ``codes * scale`` in ``dtype``."""
+    if q.is_cuda:
+        out = _binding().dequantize(q, scale, _FLOATS.get(dtype, -1))
+        if out is not None:
+            return out
     dt = _out_code(dtype)
     _codes_given(q, "q")
     device = q.device
@@ -169,6 +189,10 @@ def add_rms_norm_int8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, re
     ``x[..., K]`` and ``residual`` (same shape and type, or ``None``: then ``h`` is ``x`` itself) are fp32, bf16 or fp16;
     ``weight[K]`` any of them, or ``None`` for ones.  The norm is of the fp32 sum; ``h`` is that sum rounded to the type
     of ``x``.  ``mean`` and everything up to the codes is fp32."""
+    if x.is_cuda:
+        out = _binding().quantize(x, weight, residual, eps)
+        if out is not None:
+            return out
     dt = _float_code(x, "x")
     eps = float(eps)
     if not 0.0 <= eps < float("inf"):
@@ -224,6 +248,10 @@ def linear_int8(q: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, weig
 
     ``q[..., K]`` int8 with ``scale[...]``; ``weight[N, K]`` int8 with ``weight_scale[N]``; ``bias[N]`` or ``None``;
     ``activation`` in {none, relu, tanh}; ``dtype`` fp32, bf16 or fp16."""
+    if q.is_cuda:
+        out = _binding().linear(q, scale, weight, weight_scale, bias, _ACTS.get(activation, -1), _FLOATS.get(dtype, -1))
+        if out is not None:
+            return out
     dt = _out_code(dtype)
     act = _act_code(activation)
     _codes_given(q, "q")
@@ -258,6 +286,10 @@ def mlp3_int8(x: torch.Tensor, layers: Sequence[Tuple[torch.Tensor, torch.Tensor
     ``x[..., S]`` fp32, bf16 or fp16; ``layers``: three ``(weight[out, in] int8, weight_scale[out], bias[out] or None)``.
     The input of every layer is quantised per row; what the layers hand on is fp32; the result is in ``dtype``.  On the GPU
     the network is one launch (``mlp3_int8_kernel``) up to 2048 columns, and a launch per step beyond."""
+    if x.is_cuda and len(layers) == 3:
+        out = _binding().mlp3(x, *layers[0], *layers[1], *layers[2], _ACTS.get(final, -1), _FLOATS.get(dtype, -1))
+        if out is not None:
+            return out
     dt = _out_code(dtype)
     if len(layers) != 3:
         raise ValueError(f"three layers are expected, not {len(layers)}")
