@@ -685,7 +685,7 @@ static int launch_linear(const LinearInt8Args& a, long long kp, hipStream_t stre
     if (256 * (a.M > 1 ? a.ld_q : kp) + kp < 0x7fffffffll && 256 * (a.N > 1 ? a.ld_w : kp) + kp < 0x7fffffffll) {
         if (tiles(256) >= 192) return launch_linear_tiles<2, 2, 4, 4>(a, stream);
         if (tiles(128) >= 192) return launch_linear_tiles<2, 1, 2, 4>(a, stream);
-        if (tiles(64) >= (a.K <= 1024 ? 256 : 128)) return launch_linear_tiles<1, 1, 2, 2>(a, stream);
+        if (a.M > 32 && tiles(64) >= (a.K <= 1024 ? 256 : 128)) return launch_linear_tiles<1, 1, 2, 2>(a, stream);
     }
     const long long t = tiles(16);
     if (a.M <= 16) {
@@ -693,7 +693,7 @@ static int launch_linear(const LinearInt8Args& a, long long kp, hipStream_t stre
         if (t <= 256 && a.K >= 4096) return launch_linear_rows<1, 1, 16, 4>(a, stream);
         return launch_linear_rows<1, 1, 4, 2>(a, stream);
     }
-    if (t <= 320) return launch_linear_rows<1, 1, 4, 4>(a, stream);
+    if (t <= 320) return launch_linear_rows<1, 1, 4, 2>(a, stream);
     if (t <= 640) return launch_linear_rows<2, 1, 8, 2>(a, stream);
     if (t <= 1536) return launch_linear_rows<2, 2, 4, 4>(a, stream);
     if (a.M <= 32) return launch_linear_rows<2, 4, 4, 2>(a, stream);
@@ -732,62 +732,69 @@ __device__ __forceinline__ float load_any(const void* p, int dtype, long long i)
     return load1<_Float16>(p, i);
 }
 
-// The wave's weights, layer after layer, as one stream of units: 16 rows x 64 k (1 KB), moved from memory into the wave's
-// own ring in LDS (no registers, no barrier).  RING - 1 units are on their way ahead of the one that is multiplied, across
-// the borders of slices and layers: weights depend on nothing.  An instruction moves 16 rows of 64 neighbouring bytes in
-// lane order; read straight into the matrix operand's order, lane 16 g + c row c, the same bytes cost five times as much
-// (16 rows behind every 16 lanes: 41 us for a network of 1024 columns instead of @).
-// 16-byte pieces of a row lie XOR (row / 4): the 16 lanes of an LDS cycle then cover all banks.
+// The wave's weights, layer after layer, as one stream of slices: TPW units of 16 rows x 64 k (1 KB each), moved from
+// memory into the wave's own ring in LDS (no registers, no barrier) while the slices before are multiplied, across the
+// borders of layers too: weights depend on nothing.  An instruction moves 16 rows of 64 neighbouring bytes in lane order;
+// read straight into the matrix operand's order, lane 16 g + c row c, the same bytes keep the address path busy four times
+// as long (16 rows behind every 16 lanes).  16-byte pieces of a unit's row lie XOR (row / 4): the 16 lanes of an LDS cycle
+// then cover all banks.
+//
+// Every slice of every layer is TPW moves for every wave, so that one count says when a slice has arrived: a wide layer's
+// units are the wave's tiles at one k, a narrow layer's are one tile at TPW neighbouring k of the wave's share; what lies
+// beyond the layer repeats its last row or its last bytes and is not used.
 __device__ __forceinline__ void lds_barrier() {          // LDS is settled for the workgroup; moves stay on their way
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
-struct MlpStream {
-    int layer, slice, j;           // of the next unit to move
-    int moved, used;               // ring slots
-};
-// How a layer's units are dealt: a wave has `count` tiles tile0, tile0 + 16, ... and slices of 64 k from k0 on, `step` apart.
-struct MlpShare {
-    int K, N, tiles, count, tile0, k0, step, slices;
+struct MlpShare {                  // a wave's part of a layer: tiles tile0, tile0 + 16, ...; units of 64 k from k0, k_unit apart
+    int K, N, tiles, count, tile0, k0, k_unit, slices;
     bool narrow;
 };
+template <int TPW>
 __device__ __forceinline__ MlpShare mlp_share(const Mlp3Int8Args& a, int layer, int wave) {
     MlpShare s;
     s.K = a.width[layer], s.N = a.width[layer + 1], s.tiles = (s.N + 15) >> 4;
     s.narrow = s.tiles <= MLP_WAVES / 2;
-    const int spread = !s.narrow ? MLP_WAVES : s.tiles <= 1 ? 1 : (s.tiles <= 2 ? 2 : (s.tiles <= 4 ? 4 : 8));
-    const int parts = MLP_WAVES / spread, part = wave / spread;
-    s.tile0 = wave & (spread - 1);
-    s.count = s.tile0 < s.tiles ? (s.narrow ? 1 : (s.tiles - s.tile0 + MLP_WAVES - 1) / MLP_WAVES) : 0;
-    s.k0 = 64 * part, s.step = 64 * parts;
-    s.slices = s.count ? (s.K - s.k0 + s.step - 1) / s.step : 0;
-    if (s.slices < 0) s.slices = 0;
+    const int units = (s.K + 63) >> 6;
+    if (s.narrow) {
+        const int spread_log = s.tiles <= 1 ? 0 : (s.tiles <= 2 ? 1 : (s.tiles <= 4 ? 2 : 3)), parts = MLP_WAVES >> spread_log;
+        s.tile0 = wave & ((1 << spread_log) - 1);
+        s.count = s.tile0 < s.tiles ? 1 : 0;
+        s.k0 = 64 * (wave >> spread_log), s.k_unit = 64 * parts;
+        s.slices = (units + parts * TPW - 1) >> (4 - spread_log + (TPW == 1 ? 0 : TPW == 2 ? 1 : 2));
+    } else {
+        s.tile0 = wave, s.count = (s.tiles - wave + MLP_WAVES - 1) >> 4;
+        s.k0 = 0, s.k_unit = 0, s.slices = units;
+    }
     return s;
 }
-template <int RING>
-__device__ __forceinline__ bool mlp_move(const Mlp3Int8Args& a, MlpStream& st, MlpShare& s, signed char* ring, int wave, int lane) {
-    while (st.layer < 3 && st.slice >= s.slices) {       // the next layer that has anything for this wave
-        ++st.layer, st.slice = 0, st.j = 0;
-        if (st.layer < 3) s = mlp_share(a, st.layer, wave);
-    }
-    if (st.layer >= 3) return false;
-    const int row = lane >> 2, piece = (lane & 3) ^ (lane >> 4);
-    const int n = min(16 * (s.tile0 + MLP_WAVES * st.j) + row, s.N - 1);
-    const int k = min(s.k0 + st.slice * s.step + 16 * piece, ((s.K - 1) >> 4) << 4);
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(a.w[st.layer] + (long long)n * a.ld_w[st.layer] + k),
-                                     (__attribute__((address_space(3))) void*)(ring + st.moved * 1024), 16, 0, 0);
-    st.moved = st.moved + 1 == RING ? 0 : st.moved + 1;
-    if (++st.j == s.count) st.j = 0, ++st.slice;
-    return true;
+template <int TPW>
+struct MlpFeed {                   // the next slice to move
+    __amdgpu_buffer_rsrc_t rsrc;
+    int row[TPW];                  // this lane's row of each unit, in bytes
+    int layer, left, k, k_unit, k_step, last, slot;
+};
+template <int TPW>
+__device__ __forceinline__ void mlp_open(MlpFeed<TPW>& f, const Mlp3Int8Args& a, int wave, int lane) {
+    const MlpShare s = mlp_share<TPW>(a, f.layer, wave);
+    f.rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)a.w[f.layer], 0, 0x7fffffff, 0x00020000);
+    const int ld = (int)a.ld_w[f.layer];
+#pragma unroll
+    for (int j = 0; j < TPW; ++j) f.row[j] = min(16 * (s.tile0 + (s.narrow ? 0 : MLP_WAVES * j)) + (lane >> 2), s.N - 1) * ld;
+    f.left = s.slices, f.k = s.k0, f.k_unit = s.k_unit, f.k_step = s.narrow ? s.k_unit * TPW : 64, f.last = ((s.K - 1) >> 4) << 4;
 }
-// Moves one more unit and returns the next one's place in LDS once it has arrived.
-template <int RING>
-__device__ __forceinline__ const signed char* mlp_next(const Mlp3Int8Args& a, MlpStream& st, MlpShare& ahead, signed char* ring, int wave, int lane) {
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the slot that is moved into has been read
-    if (mlp_move<RING>(a, st, ahead, ring, wave, lane)) asm volatile("s_waitcnt vmcnt(%0)" :: "n"(RING - 1) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    const signed char* const unit = ring + st.used * 1024;
-    st.used = st.used + 1 == RING ? 0 : st.used + 1;
-    return unit;
+template <int TPW, int SLOTS>
+__device__ __forceinline__ bool mlp_move(MlpFeed<TPW>& f, const Mlp3Int8Args& a, signed char* ring, int wave, int lane) {
+    if (f.layer >= 3) return false;
+    const int piece = 16 * ((lane & 3) ^ (lane >> 4));
+    signed char* const to = ring + f.slot * (TPW * 1024);
+#pragma unroll
+    for (int j = 0; j < TPW; ++j)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(f.rsrc, (__attribute__((address_space(3))) void*)(to + j * 1024), 16,
+                                                 f.row[j] + min(f.k + j * f.k_unit + piece, f.last), 0, 0, 0);
+    f.slot = f.slot + 1 == SLOTS ? 0 : f.slot + 1;
+    f.k += f.k_step;
+    if (--f.left == 0 && ++f.layer < 3) mlp_open<TPW>(f, a, wave, lane);
+    return true;
 }
 
 // Codes of row r, columns n .. n + 3 of one lane's values.
@@ -798,20 +805,38 @@ __device__ __forceinline__ void mlp_codes(signed char* codes, int pitch, int r, 
     *reinterpret_cast<unsigned*>(codes + r * pitch + n) = pack4(b[0], b[1], b[2], b[3]);
 }
 
+// LDS of a workgroup: the waves' rings, their columns (64 scales and 64 biases each), codes, sums of narrow layers, tops.
+constexpr int mlp_slots(int tpw, int mt) { return (mt == 1 ? 8 : 6) / tpw; }
+constexpr int mlp_ring_bytes(int tpw, int mt) { return mlp_slots(tpw, mt) * tpw * 1024; }
+
 template <int TPW, int MT>
 __device__ __forceinline__ void mlp3_rows(const Mlp3Int8Args& a, signed char* const mem) {
-    constexpr int ROWS = 16 * MT, RING = MT == 1 ? 8 : 6;
+    constexpr int ROWS = 16 * MT, SLOTS = mlp_slots(TPW, MT), AHEAD = SLOTS - 1, RING = mlp_ring_bytes(TPW, MT);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     const int m0 = blockIdx.x * ROWS, pitch = a.pitch;
-    signed char* const ring = mem + wave * RING * 1024;
-    signed char* const codes = mem + MLP_WAVES * RING * 1024;
+    signed char* const ring = mem + wave * RING;
+    float* const cols = reinterpret_cast<float*>(mem + MLP_WAVES * RING) + wave * 128;
+    signed char* const codes = mem + MLP_WAVES * (RING + 512);
     int* const sums = reinterpret_cast<int*>(codes + ROWS * pitch);
     unsigned* const top = reinterpret_cast<unsigned*>(sums + a.split);       // [3][ROWS] largest magnitudes, as bits
+    const int unit = wave, ut = unit / MT, ui = unit % MT;                   // this wave's share of a narrow layer's results
 
-    MlpShare ahead = mlp_share(a, 0, wave);
-    MlpStream st = {0, 0, 0, 0, 0};
+    // scales and biases of the columns whose values this wave will make
+    auto move_columns = [&](int layer) {
+        const int N = a.width[layer + 1], tiles = (N + 15) >> 4;
+        const int tile = tiles <= MLP_WAVES / 2 ? ut : wave + MLP_WAVES * g, n = min(16 * tile + c, N - 1);
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(a.wscale[layer] + n),
+                                         (__attribute__((address_space(3))) void*)cols, 4, 0, 0);
+        if (a.bias[layer] != nullptr)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(a.bias[layer] + n),
+                                             (__attribute__((address_space(3))) void*)(cols + 64), 4, 0, 0);
+    };
+    MlpFeed<TPW> feed;
+    feed.layer = 0, feed.slot = 0;
+    mlp_open<TPW>(feed, a, wave, lane);
+    move_columns(0);
 #pragma unroll
-    for (int i = 0; i < RING - 1; ++i) mlp_move<RING>(a, st, ahead, ring, wave, lane);
+    for (int i = 0; i < AHEAD; ++i) mlp_move<TPW, SLOTS>(feed, a, ring, wave, lane);
 
     for (int i = threadIdx.x; i < a.split; i += 64 * MLP_WAVES) sums[i] = 0;
     for (int i = threadIdx.x; i < 2 * ROWS; i += 64 * MLP_WAVES) top[ROWS + i] = 0u;
@@ -823,11 +848,9 @@ __device__ __forceinline__ void mlp3_rows(const Mlp3Int8Args& a, signed char* co
             float held[HELD];
             unsigned t = 0;
 #pragma unroll
-            for (int i = 0; i < HELD; ++i) {
-                const int k = lane + 64 * i;
-                held[i] = load_any(a.x, a.xdtype, row + min(k, S - 1));
-                t = max(t, abs_bits(held[i]));   // beyond S: the last element again
-            }
+            for (int i = 0; i < HELD; ++i) held[i] = load_any(a.x, a.xdtype, row + min(lane + 64 * i, S - 1));
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) t = max(t, abs_bits(held[i]));    // beyond S: the last element again
             for (int k = lane + 64 * HELD; k < S; k += 64) t = max(t, abs_bits(load_any(a.x, a.xdtype, row + k)));
             t = wave_umax(t);
             if (lane == 0) top[r] = t;
@@ -844,33 +867,54 @@ __device__ __forceinline__ void mlp3_rows(const Mlp3Int8Args& a, signed char* co
     lds_barrier();
     const signed char* const xp = codes + c * pitch + 16 * g;
     const int wo = c * 64 + (g ^ (c >> 2)) * 16; // this lane's piece of a unit
+    int slot = 0;
     for (int layer = 0; layer < 3; ++layer) {
-        const MlpShare s = mlp_share(a, layer, wave);
+        const MlpShare s = mlp_share<TPW>(a, layer, wave);
         const int N = s.N;
-        const float* const wscale = a.wscale[layer];
-        const float* const bias = a.bias[layer];
+        const bool biased = a.bias[layer] != nullptr;
         const int act = layer < 2 ? ACT_RELU : a.act;
         const unsigned* const top_in = top + layer * ROWS;
         unsigned* const top_out = top + (layer + 1) * ROWS;
         i32x4 acc[TPW][MT] = {};
         for (int sl = 0; sl < s.slices; ++sl) {
-            i32x4 xf[MT];
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");               // the slot that is moved into has been read
+            if (mlp_move<TPW, SLOTS>(feed, a, ring, wave, lane)) asm volatile("s_waitcnt vmcnt(%0)" :: "n"(TPW * AHEAD) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            const signed char* const units = ring + slot * (TPW * 1024) + wo;
+            slot = slot + 1 == SLOTS ? 0 : slot + 1;
+            if (!s.narrow) {
+                i32x4 xf[MT], wf[TPW];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) xf[i] = *reinterpret_cast<const i32x4*>(xp + i * 16 * pitch + s.k0 + sl * s.step);
+                for (int i = 0; i < MT; ++i) xf[i] = *reinterpret_cast<const i32x4*>(xp + i * 16 * pitch + 64 * sl);
 #pragma unroll
-            for (int j = 0; j < TPW; ++j) {
-                if (j >= s.count) break;
-                const i32x4 wf = *reinterpret_cast<const i32x4*>(mlp_next<RING>(a, st, ahead, ring, wave, lane) + wo);
+                for (int j = 0; j < TPW; ++j) wf[j] = *reinterpret_cast<const i32x4*>(units + j * 1024);
 #pragma unroll
-                for (int i = 0; i < MT; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf, xf[i], acc[j][i], 0, 0, 0);
+                for (int j = 0; j < TPW; ++j)
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j], xf[i], acc[j][i], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int j = 0; j < TPW; ++j) {
+                    const int k = s.k0 + (sl * TPW + j) * s.k_unit;
+                    if (k >= s.K) break;         // the same for the wave
+                    const i32x4 wf = *reinterpret_cast<const i32x4*>(units + j * 1024);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+                        acc[0][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf, *reinterpret_cast<const i32x4*>(xp + i * 16 * pitch + k), acc[0][i], 0, 0, 0);
+                }
             }
         }
+        // The columns were moved before this layer's slices but the first AHEAD: from AHEAD slices on the waits above cover them.
+        if (s.slices < AHEAD) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         // Values of this wave: wide layers TPW x MT tiles; narrow ones the sums of all waves, dealt out again as units
-        // (tile, 16 rows), of which a wave has at most MT / 2 rounded up.
+        // (tile, 16 rows), of which a wave has at most one.
         float v[TPW][MT][4];
         unsigned m[MT] = {};
-        auto finish = [&](float (&y)[4], const i32x4 sum, int r, int n, unsigned& most) {
-            values4(y, sum, row_code(top_in[r]).scale, columns4(wscale, bias, n, N), bias != nullptr, act);
+        auto finish = [&](float (&y)[4], const i32x4 sum, int r, int n, int col, unsigned& most) {
+            Columns4 cc;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) cc.scale[e] = cols[col + e], cc.bias[e] = biased ? cols[64 + col + e] : 0.f;
+            values4(y, sum, row_code(top_in[r]).scale, cc, biased, act);
             if (layer == 2) {
                 if (m0 + r < a.M && n < N) store_values4(a.out, (long long)(m0 + r) * a.ld_out + n, a.dtype, y, N - n);
             } else {
@@ -878,7 +922,6 @@ __device__ __forceinline__ void mlp3_rows(const Mlp3Int8Args& a, signed char* co
                 for (int e = 0; e < 4; ++e) most = max(most, n + e < N ? abs_bits(y[e]) : 0u);
             }
         };
-        const int unit = wave, ut = unit / MT, ui = unit % MT;
         if (s.narrow) {
             if (s.count) {
                 int* const sum = sums + (s.tile0 * MT * 64 + lane) * 4;
@@ -892,14 +935,14 @@ __device__ __forceinline__ void mlp3_rows(const Mlp3Int8Args& a, signed char* co
                 i32x4* const from = reinterpret_cast<i32x4*>(sums + (unit * 64 + lane) * 4);
                 const i32x4 sum = *from;
                 *from = i32x4{0, 0, 0, 0};       // for the next layer that needs them
-                finish(v[0][0], sum, 16 * ui + c, 16 * ut + 4 * g, m[0]);
+                finish(v[0][0], sum, 16 * ui + c, 16 * ut + 4 * g, 4 * g, m[0]);
             }
         } else {
 #pragma unroll
             for (int j = 0; j < TPW; ++j)
                 if (j < s.count)
 #pragma unroll
-                    for (int i = 0; i < MT; ++i) finish(v[j][i], acc[j][i], 16 * i + c, 16 * (s.tile0 + MLP_WAVES * j) + 4 * g, m[i]);
+                    for (int i = 0; i < MT; ++i) finish(v[j][i], acc[j][i], 16 * i + c, 16 * (s.tile0 + MLP_WAVES * j) + 4 * g, 16 * j + 4 * g, m[i]);
         }
         if (layer == 2) break;
 #pragma unroll
@@ -910,7 +953,8 @@ __device__ __forceinline__ void mlp3_rows(const Mlp3Int8Args& a, signed char* co
             t = max(t, (unsigned)__shfl_xor((int)t, 32, 64));
             if (g == 0) atomicMax(top_out + 16 * (s.narrow ? ui : i) + c, t);
         }
-        lds_barrier();            // every wave has read the codes of this layer and given its largest
+        lds_barrier();                           // every wave has read the codes of this layer and given its largest
+        move_columns(layer + 1);
         // zeros from the layer's width up to the next slice (whole tiles write their own)
         if ((N & 63) && threadIdx.x < ROWS * 4) {
             const int n = (N & ~63) + 16 * (threadIdx.x & 3);
@@ -937,14 +981,14 @@ __global__ __launch_bounds__(64 * MLP_WAVES) void mlp3_int8_kernel(const Mlp3Int
     mlp3_rows<TPW, MT>(a, net);
 }
 
+// 1: does not fit the LDS
 template <int TPW, int MT>
-static int launch_mlp3(const Mlp3Int8Args& a, int lds, hipStream_t stream) {
+static int launch_mlp3(Mlp3Int8Args& a, int few, hipStream_t stream) {
+    a.split = few * MT * 256;
+    const int lds = MLP_WAVES * (mlp_ring_bytes(TPW, MT) + 512) + 16 * MT * a.pitch + 4 * a.split + 3 * 16 * MT * 4;
+    if (lds > 160 * 1024) return 1;
     hipLaunchKernelGGL((mlp3_int8_kernel<TPW, MT>), dim3((unsigned)((a.M + 16 * MT - 1) / (16 * MT))), dim3(64 * MLP_WAVES), lds, stream, a);
     return (int)hipGetLastError();
-}
-template <int TPW>
-static int launch_mlp3_rows(const Mlp3Int8Args& a, int mt, int lds, hipStream_t stream) {
-    return mt == 1 ? launch_mlp3<TPW, 1>(a, lds, stream) : launch_mlp3<TPW, 2>(a, lds, stream);
 }
 
 // 0: enqueued; 1: outside this kernel's range (nothing was enqueued); < 0: bad arguments.
@@ -961,25 +1005,17 @@ D4PG_API int d4pg_mlp3_int8(Mlp3Int8Args* a, hipStream_t stream) {
         const long long kp = (a->width[i] + 15) & ~15;
         if (a->w[i] == nullptr || a->wscale[i] == nullptr) return -2;
         if (((uintptr_t)a->w[i] & 15) || (a->width[i + 1] > 1 && ((a->ld_w[i] & 15) || a->ld_w[i] < kp))) return -3;
+        if (a->ld_w[i] >= 1 << 20) return 1;        // offsets inside a matrix are 32-bit
         const int tiles = (a->width[i + 1] + 15) / 16;
         if (tiles > wide_out) wide_out = tiles;
         if (tiles <= MLP_WAVES / 2 && tiles > few) few = tiles;
     }
     if (widest > 2048 || wide_out > 64) return 1;
     a->pitch = ((widest + 63) & ~63) + 16;
-    int mt = a->pad_;
-    if (mt == 0) mt = a->M <= 2048 ? 1 : 2;
-    for (;; mt /= 2) {
-        a->split = few * mt * 256;
-        const int lds = MLP_WAVES * (mt == 1 ? 8 : 6) * 1024 + 16 * mt * a->pitch + 4 * a->split + 3 * 16 * mt * 4;
-        if (lds > 160 * 1024) {
-            if (mt == 1) return 1;
-            continue;
-        }
-        if (wide_out <= 16) return launch_mlp3_rows<1>(*a, mt, lds, stream);
-        if (wide_out <= 32) return launch_mlp3_rows<2>(*a, mt, lds, stream);
-        return launch_mlp3_rows<4>(*a, mt, lds, stream);
-    }
+    const bool two = a->pad_ ? a->pad_ == 2 : a->M > 4096;        // 32 rows a workgroup
+    if (wide_out <= 16) return two ? launch_mlp3<1, 2>(*a, few, stream) : launch_mlp3<1, 1>(*a, few, stream);
+    if (wide_out <= 32) return two ? launch_mlp3<2, 2>(*a, few, stream) : launch_mlp3<2, 1>(*a, few, stream);
+    return launch_mlp3<4, 1>(*a, few, stream);
 }
 
 D4PG_SIZEOF(Mlp3Int8Args)
