@@ -782,18 +782,21 @@ __device__ __forceinline__ void mlp_open(MlpFeed<TPW>& f, const Mlp3Int8Args& a,
     for (int j = 0; j < TPW; ++j) f.row[j] = min(16 * (s.tile0 + (s.narrow ? 0 : MLP_WAVES * j)) + (lane >> 2), s.N - 1) * ld;
     f.left = s.slices, f.k = s.k0, f.k_unit = s.k_unit, f.k_step = s.narrow ? s.k_unit * TPW : 64, f.last = ((s.K - 1) >> 4) << 4;
 }
-template <int TPW, int SLOTS>
+// Moves units B BATCH .. B BATCH + BATCH - 1 of the next slice.
+template <int TPW, int BATCH, int SLOTS, int B>
 __device__ __forceinline__ bool mlp_move(MlpFeed<TPW>& f, const Mlp3Int8Args& a, signed char* ring, int wave, int lane) {
     if (f.layer >= 3) return false;
     const int piece = 16 * ((lane & 3) ^ (lane >> 4));
-    signed char* const to = ring + f.slot * (TPW * 1024);
+    signed char* const to = ring + f.slot * (BATCH * 1024);
 #pragma unroll
-    for (int j = 0; j < TPW; ++j)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(f.rsrc, (__attribute__((address_space(3))) void*)(to + j * 1024), 16,
-                                                 f.row[j] + min(f.k + j * f.k_unit + piece, f.last), 0, 0, 0);
+    for (int i = 0; i < BATCH; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(f.rsrc, (__attribute__((address_space(3))) void*)(to + i * 1024), 16,
+                                                 f.row[B * BATCH + i] + min(f.k + (B * BATCH + i) * f.k_unit + piece, f.last), 0, 0, 0);
     f.slot = f.slot + 1 == SLOTS ? 0 : f.slot + 1;
-    f.k += f.k_step;
-    if (--f.left == 0 && ++f.layer < 3) mlp_open<TPW>(f, a, wave, lane);
+    if (B == TPW / BATCH - 1) {
+        f.k += f.k_step;
+        if (--f.left == 0 && ++f.layer < 3) mlp_open<TPW>(f, a, wave, lane);
+    }
     return true;
 }
 
@@ -806,12 +809,22 @@ __device__ __forceinline__ void mlp_codes(signed char* codes, int pitch, int r, 
 }
 
 // LDS of a workgroup: the waves' rings, their columns (64 scales and 64 biases each), codes, sums of narrow layers, tops.
-constexpr int mlp_slots(int tpw, int mt) { return (mt == 1 ? 8 : 6) / tpw; }
-constexpr int mlp_ring_bytes(int tpw, int mt) { return mlp_slots(tpw, mt) * tpw * 1024; }
+// A ring holds 8 units, 6 where 32 rows of codes need the room; it is refilled BATCH units at a time.
+constexpr int mlp_ring(int mt) { return mt == 1 ? 8 : 6; }
+constexpr int mlp_batch(int tpw, int mt) { return tpw == 4 && mt == 2 ? 2 : tpw; }
+
+template <int TPW, int BATCH, int SLOTS, int I>
+__device__ __forceinline__ void mlp_ahead(MlpFeed<TPW>& f, const Mlp3Int8Args& a, signed char* ring, int wave, int lane) {
+    if constexpr (I < SLOTS - 1) {
+        mlp_move<TPW, BATCH, SLOTS, I % (TPW / BATCH)>(f, a, ring, wave, lane);
+        mlp_ahead<TPW, BATCH, SLOTS, I + 1>(f, a, ring, wave, lane);
+    }
+}
 
 template <int TPW, int MT>
 __device__ __forceinline__ void mlp3_rows(const Mlp3Int8Args& a, signed char* const mem) {
-    constexpr int ROWS = 16 * MT, SLOTS = mlp_slots(TPW, MT), AHEAD = SLOTS - 1, RING = mlp_ring_bytes(TPW, MT);
+    constexpr int ROWS = 16 * MT, BATCH = mlp_batch(TPW, MT), NB = TPW / BATCH, SLOTS = mlp_ring(MT) / BATCH, AHEAD = SLOTS - 1;
+    constexpr int RING = SLOTS * BATCH * 1024, HELD = 4;          // HELD: 64-element pieces of an input row kept in registers
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     const int m0 = blockIdx.x * ROWS, pitch = a.pitch;
     signed char* const ring = mem + wave * RING;
@@ -831,38 +844,40 @@ __device__ __forceinline__ void mlp3_rows(const Mlp3Int8Args& a, signed char* co
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(a.bias[layer] + n),
                                              (__attribute__((address_space(3))) void*)(cols + 64), 4, 0, 0);
     };
+    const int S = a.width[0];
+    float held[MT][HELD];                        // first on their way: everything waits for the input
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int p = 0; p < HELD; ++p)
+            held[i][p] = load_any(a.x, a.xdtype, (long long)min(m0 + wave + MLP_WAVES * i, a.M - 1) * a.ld_x + min(lane + 64 * p, S - 1));
     MlpFeed<TPW> feed;
     feed.layer = 0, feed.slot = 0;
     mlp_open<TPW>(feed, a, wave, lane);
     move_columns(0);
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) mlp_move<TPW, SLOTS>(feed, a, ring, wave, lane);
+    mlp_ahead<TPW, BATCH, SLOTS, 0>(feed, a, ring, wave, lane);
 
     for (int i = threadIdx.x; i < a.split; i += 64 * MLP_WAVES) sums[i] = 0;
     for (int i = threadIdx.x; i < 2 * ROWS; i += 64 * MLP_WAVES) top[ROWS + i] = 0u;
-    {
-        const int S = a.width[0], padded = (S + 63) & ~63;
-        for (int r = wave; r < ROWS; r += MLP_WAVES) {
-            const long long row = (long long)min(m0 + r, a.M - 1) * a.ld_x;
-            constexpr int HELD = 4;              // 64-element pieces of a row kept from the first pass to the second
-            float held[HELD];
-            unsigned t = 0;
+    const int padded = (S + 63) & ~63;
 #pragma unroll
-            for (int i = 0; i < HELD; ++i) held[i] = load_any(a.x, a.xdtype, row + min(lane + 64 * i, S - 1));
+    for (int i = 0; i < MT; ++i) {
+        const int r = wave + MLP_WAVES * i;
+        const long long row = (long long)min(m0 + r, a.M - 1) * a.ld_x;
+        unsigned t = 0;
 #pragma unroll
-            for (int i = 0; i < HELD; ++i) t = max(t, abs_bits(held[i]));    // beyond S: the last element again
-            for (int k = lane + 64 * HELD; k < S; k += 64) t = max(t, abs_bits(load_any(a.x, a.xdtype, row + k)));
-            t = wave_umax(t);
-            if (lane == 0) top[r] = t;
-            const RowCode rc = row_code(t);
+        for (int p = 0; p < HELD; ++p) t = max(t, abs_bits(held[i][p]));     // beyond S: the last element again
+        for (int k = lane + 64 * HELD; k < S; k += 64) t = max(t, abs_bits(load_any(a.x, a.xdtype, row + k)));
+        t = wave_umax(t);
+        if (lane == 0) top[r] = t;
+        const RowCode rc = row_code(t);
 #pragma unroll
-            for (int i = 0; i < HELD; ++i) {
-                const int k = lane + 64 * i;
-                if (k < padded) codes[r * pitch + k] = k < S ? (signed char)(code_bits(held[i], rc) & rc.keep) : 0;
-            }
-            for (int k = lane + 64 * HELD; k < padded; k += 64)
-                codes[r * pitch + k] = k < S ? (signed char)(code_bits(load_any(a.x, a.xdtype, row + k), rc) & rc.keep) : 0;
+        for (int p = 0; p < HELD; ++p) {
+            const int k = lane + 64 * p;
+            if (k < padded) codes[r * pitch + k] = k < S ? (signed char)(code_bits(held[i][p], rc) & rc.keep) : 0;
         }
+        for (int k = lane + 64 * HELD; k < padded; k += 64)
+            codes[r * pitch + k] = k < S ? (signed char)(code_bits(load_any(a.x, a.xdtype, row + k), rc) & rc.keep) : 0;
     }
     lds_barrier();
     const signed char* const xp = codes + c * pitch + 16 * g;
@@ -877,35 +892,43 @@ __device__ __forceinline__ void mlp3_rows(const Mlp3Int8Args& a, signed char* co
         unsigned* const top_out = top + (layer + 1) * ROWS;
         i32x4 acc[TPW][MT] = {};
         for (int sl = 0; sl < s.slices; ++sl) {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");               // the slot that is moved into has been read
-            if (mlp_move<TPW, SLOTS>(feed, a, ring, wave, lane)) asm volatile("s_waitcnt vmcnt(%0)" :: "n"(TPW * AHEAD) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            const signed char* const units = ring + slot * (TPW * 1024) + wo;
-            slot = slot + 1 == SLOTS ? 0 : slot + 1;
+            i32x4 xf[MT];
             if (!s.narrow) {
-                i32x4 xf[MT], wf[TPW];
 #pragma unroll
                 for (int i = 0; i < MT; ++i) xf[i] = *reinterpret_cast<const i32x4*>(xp + i * 16 * pitch + 64 * sl);
-#pragma unroll
-                for (int j = 0; j < TPW; ++j) wf[j] = *reinterpret_cast<const i32x4*>(units + j * 1024);
-#pragma unroll
-                for (int j = 0; j < TPW; ++j)
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j], xf[i], acc[j][i], 0, 0, 0);
-            } else {
-#pragma unroll
-                for (int j = 0; j < TPW; ++j) {
-                    const int k = s.k0 + (sl * TPW + j) * s.k_unit;
-                    if (k >= s.K) break;         // the same for the wave
-                    const i32x4 wf = *reinterpret_cast<const i32x4*>(units + j * 1024);
-#pragma unroll
-                    for (int i = 0; i < MT; ++i)
-                        acc[0][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf, *reinterpret_cast<const i32x4*>(xp + i * 16 * pitch + k), acc[0][i], 0, 0, 0);
-                }
             }
+            auto batch = [&](auto b_c) {
+                constexpr int B = decltype(b_c)::value;
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // the slot that is moved into has been read
+                if (mlp_move<TPW, BATCH, SLOTS, (B + AHEAD) % NB>(feed, a, ring, wave, lane)) asm volatile("s_waitcnt vmcnt(%0)" :: "n"(BATCH * AHEAD) : "memory");
+                else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                const signed char* const units = ring + slot * (BATCH * 1024) + wo;
+                slot = slot + 1 == SLOTS ? 0 : slot + 1;
+                if (!s.narrow) {
+                    i32x4 wf[BATCH];
+#pragma unroll
+                    for (int j = 0; j < BATCH; ++j) wf[j] = *reinterpret_cast<const i32x4*>(units + j * 1024);
+#pragma unroll
+                    for (int j = 0; j < BATCH; ++j)
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) acc[B * BATCH + j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j], xf[i], acc[B * BATCH + j][i], 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < BATCH; ++j) {
+                        const int k = s.k0 + (sl * TPW + B * BATCH + j) * s.k_unit;
+                        if (k >= s.K) break;     // the same for the wave
+                        const i32x4 wf = *reinterpret_cast<const i32x4*>(units + j * 1024);
+#pragma unroll
+                        for (int i = 0; i < MT; ++i)
+                            acc[0][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf, *reinterpret_cast<const i32x4*>(xp + i * 16 * pitch + k), acc[0][i], 0, 0, 0);
+                    }
+                }
+            };
+            batch(std::integral_constant<int, 0>());
+            if constexpr (NB == 2) batch(std::integral_constant<int, 1>());
         }
-        // The columns were moved before this layer's slices but the first AHEAD: from AHEAD slices on the waits above cover them.
-        if (s.slices < AHEAD) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        // The columns were moved before this layer's batches but the first AHEAD: from AHEAD batches on the waits above cover them.
+        if (s.slices * NB < AHEAD) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         // Values of this wave: wide layers TPW x MT tiles; narrow ones the sums of all waves, dealt out again as units
         // (tile, 16 rows), of which a wave has at most one.
         float v[TPW][MT][4];
@@ -924,17 +947,18 @@ __device__ __forceinline__ void mlp3_rows(const Mlp3Int8Args& a, signed char* co
         };
         if (s.narrow) {
             if (s.count) {
-                int* const sum = sums + (s.tile0 * MT * 64 + lane) * 4;
+                int* const sum = sums + s.tile0 * MT * 256 + lane;
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) atomicAdd(sum + i * 256 + e, acc[0][i][e]);
+                    for (int e = 0; e < 4; ++e) atomicAdd(sum + i * 256 + e * 64, acc[0][i][e]);
             }
             lds_barrier();
             if (ut < s.tiles) {
-                i32x4* const from = reinterpret_cast<i32x4*>(sums + (unit * 64 + lane) * 4);
-                const i32x4 sum = *from;
-                *from = i32x4{0, 0, 0, 0};       // for the next layer that needs them
+                int* const from = sums + unit * 256 + lane;
+                i32x4 sum;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[e] = from[e * 64], from[e * 64] = 0;   // zeros for the next layer that needs them
                 finish(v[0][0], sum, 16 * ui + c, 16 * ut + 4 * g, 4 * g, m[0]);
             }
         } else {
@@ -985,7 +1009,7 @@ __global__ __launch_bounds__(64 * MLP_WAVES) void mlp3_int8_kernel(const Mlp3Int
 template <int TPW, int MT>
 static int launch_mlp3(Mlp3Int8Args& a, int few, hipStream_t stream) {
     a.split = few * MT * 256;
-    const int lds = MLP_WAVES * (mlp_ring_bytes(TPW, MT) + 512) + 16 * MT * a.pitch + 4 * a.split + 3 * 16 * MT * 4;
+    const int lds = MLP_WAVES * (mlp_ring(MT) * 1024 + 512) + 16 * MT * a.pitch + 4 * a.split + 3 * 16 * MT * 4;
     if (lds > 160 * 1024) return 1;
     hipLaunchKernelGGL((mlp3_int8_kernel<TPW, MT>), dim3((unsigned)((a.M + 16 * MT - 1) / (16 * MT))), dim3(64 * MLP_WAVES), lds, stream, a);
     return (int)hipGetLastError();
@@ -1015,6 +1039,7 @@ D4PG_API int d4pg_mlp3_int8(Mlp3Int8Args* a, hipStream_t stream) {
     const bool two = a->pad_ ? a->pad_ == 2 : a->M > 4096;        // 32 rows a workgroup
     if (wide_out <= 16) return two ? launch_mlp3<1, 2>(*a, few, stream) : launch_mlp3<1, 1>(*a, few, stream);
     if (wide_out <= 32) return two ? launch_mlp3<2, 2>(*a, few, stream) : launch_mlp3<2, 1>(*a, few, stream);
+    if (two) return launch_mlp3<4, 2>(*a, few, stream);
     return launch_mlp3<4, 1>(*a, few, stream);
 }
 
