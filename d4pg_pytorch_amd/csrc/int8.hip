@@ -401,11 +401,6 @@ D4PG_API int d4pg_dequant_rows(DequantRowsArgs* a, hipStream_t stream) {
 // product of codes
 // ---------------------------------------------------------------------------------------------------------------
 
-__device__ __forceinline__ float act_of(float y, int act) {
-    if (act == ACT_RELU) return y < 0.f ? 0.f : y;        // keeps NaN
-    if (act == ACT_TANH) return tanhf(y);
-    return y;
-}
 // Four neighbouring columns n .. n + 3 of row m (those below N).  v: integer sums.
 template <typename T>
 __device__ __forceinline__ void store4(T* out, const float (&v)[4], int left) {
@@ -434,14 +429,23 @@ __device__ __forceinline__ Columns4 columns4(const float* wscale, const float* b
     }
     return c;
 }
-// act(sum * s * t + b) of four columns.  ONE definition, contraction off: every kernel below rounds alike.
-__device__ __forceinline__ void values4(float (&v)[4], const i32x4 sum, float sm, const Columns4& c, bool biased, int act) {
+// act(scaled * t + b) of four columns, scaled = sum * s.  ONE definition, contraction off: every kernel below rounds alike.
+__device__ __forceinline__ f32x4 scaled4(const i32x4 sum, float sm) {
+    return f32x4{(float)sum[0] * sm, (float)sum[1] * sm, (float)sum[2] * sm, (float)sum[3] * sm};
+}
+__device__ __forceinline__ void values4(float (&v)[4], const f32x4 scaled, const Columns4& c, bool biased, int act) {
 #pragma clang fp contract(off)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        v[i] = ((float)sum[i] * sm) * c.scale[i];
+        v[i] = scaled[i] * c.scale[i];
         if (biased) v[i] += c.bias[i];
-        v[i] = act_of(v[i], act);
+    }
+    if (act == ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];       // keeps NaN
+    } else if (act == ACT_TANH) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = tanhf(v[i]);
     }
 }
 __device__ __forceinline__ void store_values4(void* out, long long at, int dtype, const float (&v)[4], int left) {
@@ -449,10 +453,10 @@ __device__ __forceinline__ void store_values4(void* out, long long at, int dtype
     else if (dtype == F_BF16) store4(reinterpret_cast<__bf16*>(out) + at, v, left);
     else store4(reinterpret_cast<_Float16*>(out) + at, v, left);
 }
-__device__ __forceinline__ void finish4(const LinearInt8Args& a, int m, int n, const i32x4 sum, float sm, const Columns4& c) {
+__device__ __forceinline__ void finish4(const LinearInt8Args& a, int m, int n, const f32x4 scaled, const Columns4& c) {
     if (m >= a.M || n >= a.N) return;
     float v[4];
-    values4(v, sum, sm, c, a.bias != nullptr, a.act);
+    values4(v, scaled, c, a.bias != nullptr, a.act);
     store_values4(a.out, (long long)m * a.ld_out + n, a.dtype, v, a.N - n);
 }
 
@@ -486,6 +490,16 @@ __global__ __launch_bounds__(64 * WAVES) void linear_int8_rows_kernel(const Line
 #pragma unroll
     for (int i = 0; i < NT; ++i) wp[i] = a.w + (long long)min((tn * NT + i) * 16 + c, a.N - 1) * a.ld_w;
     const int last = ((a.K - 1) >> 4) << 4;      // the last 16 bytes of a row that hold a code
+    // what the results of this wave need besides their sums: asked for before the products, not after them
+    constexpr int MINE = (MT * NT + WAVES - 1) / WAVES;
+    float sm[MINE];
+    Columns4 col[MINE];
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+        const int u = min(wave + i * WAVES, MT * NT - 1);
+        sm[i] = a.scale[min((tm * MT + u / NT) * 16 + c, a.M - 1)];
+        col[i] = columns4(a.wscale, a.bias, (tn * NT + u % NT) * 16 + 4 * g, a.N);
+    }
     i32x4 acc[MT][NT] = {};
     // slice s of the wave covers k = 64 (wave + s WAVES): neighbouring waves read neighbouring bytes
     for (int k0 = 64 * wave; k0 < a.K; k0 += 64 * WAVES * U) {
@@ -518,12 +532,14 @@ __global__ __launch_bounds__(64 * WAVES) void linear_int8_rows_kernel(const Line
 #pragma unroll
         for (int j = 0; j < NT; ++j) part[wave][i * NT + j][lane] = acc[i][j];
     __syncthreads();
-    for (int u = wave; u < MT * NT; u += WAVES) {
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+        const int u = wave + i * WAVES;
+        if (u >= MT * NT) break;
         i32x4 sum = part[0][u][lane];
 #pragma unroll
         for (int w = 1; w < WAVES; ++w) sum += part[w][u][lane];
-        const int m = (tm * MT + u / NT) * 16 + c, n = (tn * NT + u % NT) * 16 + 4 * g;
-        finish4(a, m, n, sum, a.scale[min(m, a.M - 1)], columns4(a.wscale, a.bias, n, a.N));
+        finish4(a, (tm * MT + u / NT) * 16 + c, (tn * NT + u % NT) * 16 + 4 * g, scaled4(sum, sm[i]), col[i]);
     }
 }
 
@@ -553,14 +569,14 @@ static int launch_linear_rows(const LinearInt8Args& a, hipStream_t stream) {
 // What bounds it at 8192^3 (tiles of 256): power first - the matrix instruction alone does 4.9 P/s on zeros, 3.5 on random
 // codes, 3.1 - 3.2 with its LDS reads - then how well the rest hides behind it.  Moves alone take 231 us.  Waves a SIMD
 // decide the rest: 1 (waves of 128 x 128) 560 us, matrix pipe 52 % busy; 2 (128 x 64) 476; 4 (64 x 64) 464 us = 2.37 P/s.
-enum { STEP_LOAD = 0, STEP_READ = 1, STEP_LAST = 2 };
+enum { STEP_FULL = 0, STEP_DRAIN = 1, STEP_LAST = 2 };
 
-template <int MI, int NI, int WM, int WN>
+template <int MI, int NI, int WM, int WN, int KW, int S>
 __device__ __forceinline__ void linear_tile(const LinearInt8Args& a, signed char* const lds) {
     constexpr int BM = 32 * MI * WM, BN = 32 * NI * WN, TILE = (BM + BN) * 128, GROUP = 2048 / BM;
-    constexpr int MOVES = (BM + BN) / 8 / (WM * WN);
+    constexpr int MOVES = (BM + BN) / 8 / (WM * WN * KW), SLICES = 4 / KW;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave % WM, wn = wave / WM, r = lane & 31, h = lane >> 5;
+    const int wm = wave % WM, wn = wave / WM % WN, wk = wave / (WM * WN), r = lane & 31, h = lane >> 5;
 
     const int tiles_m = (a.M + BM - 1) / BM, tiles_n = (a.N + BN - 1) / BN, total = tiles_m * tiles_n;
     const int xcd = blockIdx.x & 7, share = total >> 3, rest = total & 7;
@@ -581,111 +597,150 @@ __device__ __forceinline__ void linear_tile(const LinearInt8Args& a, signed char
     const int piece[2] = {((lane & 7) ^ (lane >> 4)) * 16, ((lane & 7) ^ (4 + (lane >> 4))) * 16}, last = ((a.K - 1) >> 4) << 4;
     auto load = [&](int t) {
         const int k[2] = {min(t * 128 + piece[0], last), min(t * 128 + piece[1], last)};
-        signed char* const to = lds + (t & 1) * TILE + row0 * 128;
+        signed char* const to = lds + (t & (S - 1)) * TILE + row0 * 128;
 #pragma unroll
         for (int i = 0; i < MOVES; ++i)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(to + i * 1024), 16, off[i] + k[i & 1], 0, 0, 0);
     };
     i32x4 fx[2][MI], fw[2][NI];
-    auto read = [&](int t, int ks, int b) {
-        const signed char* const at = lds + (t & 1) * TILE + ((2 * ks + h) ^ ((lane >> 1) & 7)) * 16;
+    auto read = [&](int t, int sl, int b) {       // slice sl of the wave's SLICES
+        const signed char* const at = lds + (t & (S - 1)) * TILE + ((2 * (wk * SLICES + sl) + h) ^ ((lane >> 1) & 7)) * 16;
 #pragma unroll
         for (int i = 0; i < NI; ++i) fw[b][i] = *reinterpret_cast<const i32x4*>(at + (BM + wn * 32 * NI + i * 32 + r) * 128);
 #pragma unroll
         for (int i = 0; i < MI; ++i) fx[b][i] = *reinterpret_cast<const i32x4*>(at + (wm * 32 * MI + i * 32 + r) * 128);
     };
     i32x16 acc[NI][MI] = {};
+    float sm[MI];                                 // the rows' scales: here, where the moves hide their way
+#pragma unroll
+    for (int j = 0; j < MI; ++j) sm[j] = a.scale[min(m0 + wm * 32 * MI + j * 32 + r, a.M - 1)];
+    const int steps = (a.K + 127) >> 7;
     auto step = [&](int t, auto mode_c) {
         constexpr int MODE = decltype(mode_c)::value;
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-            if (ks < 3) {
-                read(t, ks + 1, (ks + 1) & 1);
+        for (int sl = 0; sl < SLICES; ++sl) {
+            if (sl < SLICES - 1) {
+                read(t, sl + 1, (sl + 1) & 1);
             } else if (MODE != STEP_LAST) {
-                __syncthreads();                  // step t + 1 has arrived, step t has been read by every wave
+                // step t + 1 has arrived, step t has been read by every wave
+                if (MODE == STEP_FULL) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(MOVES * (S - 2)) : "memory");
+                else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
                 read(t + 1, 0, 0);
-                if (MODE == STEP_LOAD) load(t + 2);
+                if (MODE == STEP_FULL && t + S < steps) load(t + S);
             }
             if (MODE == STEP_LAST) {
-                const i32x4 mask = below(t * 128 + ks * 32 + h * 16, a.K);
+                const i32x4 mask = below(t * 128 + (wk * SLICES + sl) * 32 + h * 16, a.K);
 #pragma unroll
-                for (int j = 0; j < MI; ++j) fx[ks & 1][j] &= mask;
+                for (int j = 0; j < MI; ++j) fx[sl & 1][j] &= mask;
             }
 #pragma unroll
             for (int i = 0; i < NI; ++i)
 #pragma unroll
-                for (int j = 0; j < MI; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[ks & 1][i], fx[ks & 1][j], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < MI; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[sl & 1][i], fx[sl & 1][j], acc[i][j], 0, 0, 0);
         }
     };
-    const int steps = (a.K + 127) >> 7;
-    load(0);
-    __syncthreads();
-    if (steps > 1) load(1);
+    for (int t = 0; t < S && t < steps; ++t) load(t);
+    if (steps >= S) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "n"(MOVES * (S - 1)) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     read(0, 0, 0);
-    for (int t = 0; t < steps - 2; ++t) step(t, std::integral_constant<int, STEP_LOAD>());
-    if (steps > 1) step(steps - 2, std::integral_constant<int, STEP_READ>());
+    int t = 0;
+    for (; t <= steps - S; ++t) {
+        if (t == steps - 1) break;                // S = 1 step
+        step(t, std::integral_constant<int, STEP_FULL>());
+    }
+    for (; t < steps - 1; ++t) step(t, std::integral_constant<int, STEP_DRAIN>());
     step(steps - 1, std::integral_constant<int, STEP_LAST>());
 
     // Element 4 e + i of an accumulator is column 8 e + 4 h + i of its 32, row r.  32 rows of the wave at a time go through
-    // LDS (its own part of it; rows 16 bytes apart from a bank's multiple), so that a row's columns leave side by side.
+    // LDS, times their scale (its own part of it; rows 16 bytes apart from a bank's multiple), so that a row's columns leave
+    // side by side.
     constexpr int PITCH = 32 * NI + 4, LANES = 8 * NI;            // words of a row; lanes that write one row of 4 columns each
-    int* const stage = reinterpret_cast<int*>(lds) + wave * 32 * PITCH;
+    __syncthreads();
+    if (KW == 2) {                                // the second half of K joins the first
+        i32x4* const half = reinterpret_cast<i32x4*>(lds) + wave % (WM * WN) * (NI * MI * 256) + lane;
+#pragma unroll
+        for (int i = 0; i < NI * MI * 4; ++i) {
+            const i32x16& v = acc[i / 4 / MI][i / 4 % MI];
+            if (wk == 1) half[i * 64] = i32x4{v[4 * (i % 4)], v[4 * (i % 4) + 1], v[4 * (i % 4) + 2], v[4 * (i % 4) + 3]};
+        }
+        __syncthreads();
+        if (wk == 1) return;                      // nothing below waits for another wave
+#pragma unroll
+        for (int i = 0; i < NI * MI * 4; ++i) {
+            const i32x4 v = half[i * 64];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i / 4 / MI][i / 4 % MI][4 * (i % 4) + e] += v[e];
+        }
+    }
+    // (KW == 2: behind the halves, which other waves may still be reading)
+    float* const stage = reinterpret_cast<float*>(lds + (KW == 2 ? WM * WN * NI * MI * 4096 : 0)) + wave * 32 * PITCH;
     const int n = n0 + wn * 32 * NI + lane % LANES * 4;
     const Columns4 col = columns4(a.wscale, a.bias, n, a.N);
-    __syncthreads();
 #pragma unroll
     for (int j = 0; j < MI; ++j) {
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const i32x4 sum = {acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
-                *reinterpret_cast<i32x4*>(stage + r * PITCH + i * 32 + 8 * e + 4 * h) = sum;
+                f32x4 v;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) v[x] = (float)acc[i][j][4 * e + x] * sm[j];
+                *reinterpret_cast<f32x4*>(stage + r * PITCH + i * 32 + 8 * e + 4 * h) = v;
             }
         __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
+#pragma unroll 2
         for (int row = lane / LANES; row < 32; row += 64 / LANES) {
             const int m = m0 + wm * 32 * MI + j * 32 + row;
-            const i32x4 sum = *reinterpret_cast<const i32x4*>(stage + row * PITCH + lane % LANES * 4);
-            finish4(a, m, n, sum, a.scale[min(m, a.M - 1)], col);
+            const f32x4 scaled = *reinterpret_cast<const f32x4*>(stage + row * PITCH + lane % LANES * 4);
+            finish4(a, m, n, scaled, col);
         }
         __builtin_amdgcn_wave_barrier();
     }
 }
 
-template <int MI, int NI, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN, WM * WN / 4 * (MI * NI * WM * WN > 32 ? 1 : 2)) void linear_int8_tiles_kernel(const LinearInt8Args a) {
+template <int MI, int NI, int WM, int WN, int KW, int S>
+__global__ __launch_bounds__(64 * WM * WN * KW, WM * WN * KW / 4 * (MI * NI * WM * WN > 32 ? 1 : 2)) void linear_int8_tiles_kernel(const LinearInt8Args a) {
     extern __shared__ __attribute__((aligned(128))) signed char tiles[];
-    linear_tile<MI, NI, WM, WN>(a, tiles);
+    linear_tile<MI, NI, WM, WN, KW, S>(a, tiles);
 }
 
-template <int MI, int NI, int WM, int WN>
+template <int MI, int NI, int WM, int WN, int KW, int S>
 static int launch_linear_tiles(const LinearInt8Args& a, hipStream_t stream) {
-    constexpr int BM = 32 * MI * WM, BN = 32 * NI * WN, TILES = 2 * (BM + BN) * 128, STAGE = WM * WN * 32 * (32 * NI + 4) * 4;
+    constexpr int BM = 32 * MI * WM, BN = 32 * NI * WN, TILES = S * (BM + BN) * 128, STAGE = WM * WN * (32 * (32 * NI + 4) * 4 + (KW == 2 ? NI * MI * 4096 : 0));
     constexpr int LDS = TILES > STAGE ? TILES : STAGE;
     const long long tiles = (long long)((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN);
     if (tiles > 0x7fffffffll) return -7;
-    hipLaunchKernelGGL((linear_int8_tiles_kernel<MI, NI, WM, WN>), dim3((unsigned)tiles), dim3(64 * WM * WN), LDS, stream, a);
+    hipLaunchKernelGGL((linear_int8_tiles_kernel<MI, NI, WM, WN, KW, S>), dim3((unsigned)tiles), dim3(64 * WM * WN * KW), LDS, stream, a);
     return (int)hipGetLastError();
 }
 
 // Which kernel.  Tiles are taken from the largest size that still gives most of the 256 CUs one; below 128 tiles of 64 x 64
-// (256 where K is short: a tile then ends before its moves have paid) the rows kernel, whose workgroups split K instead.
-// Measured on an MI355X, us (graph of 20 calls, median), the other choice behind the /:
-//     256 x 256, 16 waves    2048 x 8192 x 8192 (256 tiles)  132 / 158 (128 x 128)    2048 x 4096 x 4096 (128)  54 / 45
-//     128 x 128, 8 waves     4096 x 1024 x 1024 (256)        13.8 / 13.4 (64 x 64)    512 x 4096 x 4096 (128)   24.8 / 18.9
-//     64 x 64, 4 waves       256 x 4096 x 4096 (256)         12.7 / 25 (rows)         512 x 1024 x 1024 (128)   6.7 / 6.3
+// (256 where K is short: a tile then ends before its moves have paid) and up to 32 rows the rows kernel, whose workgroups
+// split K instead.  A size whose tiles fit the CUs at once gets a workgroup to itself: four steps of moves in flight and
+// more waves for the same tile; beyond that two workgroups a CU hide each other's waits.
+// Measured on an MI355X, us (graph of 20 calls, median):
+//     tile, waves, steps in LDS   for                            and by the neighbouring choice
+//     256 x 256, 16, 2            2048 x 8192 x 8192  (256)  132   158 with 128 x 128;  2048 x 4096 x 4096 (128 tiles)  54 / 45
+//     128 x 128, 16, 4            1024 x 4096 x 4096  (256)   25   29 with 8 waves, 2 steps;  2048 x 4096 x 4096 (512)  52 / 45
+//     128 x 128,  8, 2            8192 x 1024 x 1024  (512)   18   22 with 16 waves, 4 steps; 26 with 256 x 256
+//     64 x 64, 8 on half of K, 4  256 x 4096 x 4096   (256)   11.5 12.8 with 4 waves, 2 steps; 25 with rows
+//     64 x 64,  4, 2              2048 x 1024 x 1024  (512)    7.5 8.2 with K halved; 10.1 with 128 x 128
+//     rows                        512 x 1024 x 1024   (128)    6.2 6.3 with 64 x 64;  128 x 4096 x 4096 (128)  14.1 / 10.8
 // Between the row kernels the number of 16 x 16 tiles decides: as many columns and rows a workgroup as leave 200 - 400
 // workgroups (256 x 400 x 400: 3.7 with 2 x 1 tiles, 4.0 with 1 x 1, 4.2 with 2 x 2; 512 x 1024 x 1024: 6.3 with 4 x 2, 6.9
-// with 2 x 2, 8.6 with 2 x 1; 1 x 16384 x 4096: 13.9 with 1 x 4, 15.2 with 1 x 1), and K is dealt to 16 waves where it is long
-// and the workgroups are few (1 x 4096 x 4096: 5.6 with 16 waves, 6.6 with 4; 1 x 1333 x 2001: 4.4 and 3.6).
+// with 2 x 2, 8.6 with 2 x 1; 1 x 16384 x 4096: 12.8 with 1 x 4, 14.6 with 1 x 1), and K is dealt to 16 waves where it is long
+// and the workgroups are few (1 x 4096 x 4096: 5.5 with 16 waves, 6.5 with 4; 1 x 1333 x 2001: 4.4 and 3.6).
 static int launch_linear(const LinearInt8Args& a, long long kp, hipStream_t stream) {
     auto tiles = [&](int side) { return (long long)((a.M + side - 1) / side) * ((a.N + side - 1) / side); };
     // the tile kernel's offsets inside 256 rows are 32-bit
     if (256 * (a.M > 1 ? a.ld_q : kp) + kp < 0x7fffffffll && 256 * (a.N > 1 ? a.ld_w : kp) + kp < 0x7fffffffll) {
-        if (tiles(256) >= 192) return launch_linear_tiles<2, 2, 4, 4>(a, stream);
-        if (tiles(128) >= 192) return launch_linear_tiles<2, 1, 2, 4>(a, stream);
-        if (a.M > 32 && tiles(64) >= (a.K <= 1024 ? 256 : 128)) return launch_linear_tiles<1, 1, 2, 2>(a, stream);
+        if (tiles(256) >= 192) return launch_linear_tiles<2, 2, 4, 4, 1, 2>(a, stream);
+        if (tiles(128) > 256) return launch_linear_tiles<2, 1, 2, 4, 1, 2>(a, stream);
+        if (tiles(128) >= 192) return launch_linear_tiles<1, 1, 4, 4, 1, 4>(a, stream);
+        if (a.M > 32 && tiles(64) >= (a.K <= 1024 ? 256 : 128)) {
+            if (tiles(64) <= 256 || a.K >= 4096) return launch_linear_tiles<1, 1, 2, 2, 2, 4>(a, stream);
+            return launch_linear_tiles<1, 1, 2, 2, 1, 2>(a, stream);
+        }
     }
     const long long t = tiles(16);
     if (a.M <= 16) {
@@ -937,7 +992,7 @@ __device__ __forceinline__ void mlp3_rows(const Mlp3Int8Args& a, signed char* co
             Columns4 cc;
 #pragma unroll
             for (int e = 0; e < 4; ++e) cc.scale[e] = cols[col + e], cc.bias[e] = biased ? cols[64 + col + e] : 0.f;
-            values4(y, sum, row_code(top_in[r]).scale, cc, biased, act);
+            values4(y, scaled4(sum, row_code(top_in[r]).scale), cc, biased, act);
             if (layer == 2) {
                 if (m0 + r < a.M && n < N) store_values4(a.out, (long long)(m0 + r) * a.ld_out + n, a.dtype, y, N - n);
             } else {

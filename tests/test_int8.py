@@ -225,7 +225,10 @@ def _check_linear(y, q, scale, w, ws, b, act, dtype):
 
 SHAPES = [(1, 1, 1), (1, 3, 15), (2, 4, 16), (1, 400, 400), (3, 5, 17), (16, 16, 64), (17, 33, 65), (1, 50, 1000), (5, 17, 127),
           (31, 31, 129), (64, 51, 400), (65, 64, 256), (128, 128, 128), (129, 130, 131), (256, 400, 400), (300, 7, 2001),
-          (7, 300, 2001), (257, 513, 640), (500, 260, 1111), (2, 4096, 1024), (1030, 1025, 385), (40, 2050, 96)]
+          (7, 300, 2001), (257, 513, 640), (500, 260, 1111), (2, 4096, 1024), (1030, 1025, 385), (40, 2050, 96),
+          # one shape at least for every tile size and row kernel, all with ragged edges
+          (3585, 3333, 300), (2300, 1700, 1300), (1793, 1665, 700), (700, 900, 5000), (150, 4000, 4100), (130, 4090, 1100), (1000, 1030, 1023),
+          (16, 12300, 200), (3, 12289, 70), (9, 3000, 4100), (30, 7000, 333), (31, 20000, 50), (60, 3100, 77), (900, 300, 1000), (17, 330, 128)]
 
 
 @pytest.mark.parametrize("device", DEVICES)
