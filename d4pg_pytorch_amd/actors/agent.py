@@ -37,7 +37,8 @@ def make_policy(config: Dict, device: str):
     if str(device).startswith("cuda"):
         from .gpu_actor import GpuActor
         return GpuActor(config["state_dim"], config["action_dim"], config["dense_size"],
-                        max_batch=max(1, int(config.get("envs_per_agent", 1))), device=device, action_scale=scale)
+                        max_batch=max(1, int(config.get("envs_per_agent", 1))), device=device, action_scale=scale,
+                        precision=config.get("policy_precision", "fp32"))
     return CpuActor(config["state_dim"], config["action_dim"], config["dense_size"], action_scale=scale)
 
 

@@ -17,6 +17,9 @@ rebuilt on the device (``pack_actor32_kernel``) from flat fp32 parameters that a
 
 Hidden widths outside the fused kernel's set fall back to three launches of the per-layer fp32 MFMA
 GEMM (``csrc/gemm.hip``).
+
+``precision="int8"`` answers with 8-bit codes instead: the weights are quantised per output channel whenever new
+parameters arrive, states and hidden activations per row (``ops/int8.py::mlp3_int8``, one launch up to 1024 columns).
 """
 from __future__ import annotations
 
@@ -29,6 +32,7 @@ import torch
 
 from ..models.nets import NetLayout, NetView, Packed32, pad4, pad16, pad32
 from ..ops import hip as H
+from ..ops.int8 import mlp3_int8, quantize_rows
 
 LDS_PAD32 = 4
 #: states per launch from which the policy runs on the 16x16x4 kernel, as the learner's phases do (models/hip_core_f32.py):
@@ -128,8 +132,11 @@ class PackedActor32:
 
 class GpuActor:
     def __init__(self, state_dim: int, action_dim: int, hidden: int, max_batch: int = 1,
-                 device="cuda", action_scale: float = 1.0):
+                 device="cuda", action_scale: float = 1.0, precision: str = "fp32"):
+        if precision not in ("fp32", "int8"):
+            raise ValueError(f"precision must be 'fp32' or 'int8', not {precision!r}")
         H.lib()
+        self.precision = precision
         self.S, self.A, self.Hd, self.E = state_dim, action_dim, hidden, int(max_batch)
         self.device = torch.device(device)
         self.layout = NetLayout.build(state_dim, hidden, action_dim)
@@ -144,20 +151,29 @@ class GpuActor:
         self._out_host = torch.zeros(self.E, lda).pin_memory()
         self._flat_host = torch.zeros(self.layout.numel).pin_memory()
         self.fused = PackedActor32(state_dim, action_dim, hidden, self.device, rows=self.E) \
-            if PackedActor32.supported(state_dim, action_dim, hidden) else None
-        if self.fused is None:         # per-layer path: two hidden activation buffers
+            if precision == "fp32" and PackedActor32.supported(state_dim, action_dim, hidden) else None
+        self.codes = None              # int8: three (weight codes, scales, bias)
+        if precision == "int8":
+            self._quantize()
+        elif self.fused is None:         # per-layer path: two hidden activation buffers
             self.h1 = torch.zeros(self.E, ldh, device=self.device)
             self.h2 = torch.zeros(self.E, ldh, device=self.device)
-        self.launches_per_act = 1 if self.fused is not None else 3
+        self.launches_per_act = 1 if self.fused is not None else (2 if precision == "int8" else 3)
         self._shared = None
         self._shared_half = 0
 
     # ------------------------------------------------------------------ weights
+    def _quantize(self) -> None:
+        """Codes of the parameters in ``flat``, per output channel.  Enqueue only."""
+        self.codes = tuple((*quantize_rows(w), b) for w, b in zip(self.view.weights, self.view.biases))
+
     def load_flat(self, flat) -> None:
         self._flat_host.copy_(torch.as_tensor(np.asarray(flat, dtype=np.float32)))
         self.flat.copy_(self._flat_host, non_blocking=True)
         if self.fused is not None:
             self.fused.pack_from(self.flat.data_ptr())
+        elif self.codes is not None:
+            self._quantize()
 
     def attach_shared(self, shared, actor_index: int) -> None:
         """Follow the learner's weights in place.  ``shared`` is the learner's ``SharedDeviceBuffer``: two
@@ -176,6 +192,8 @@ class GpuActor:
         self.flat.copy_(self._shared.tensor[base: base + n], non_blocking=True)      # for state_dict() / checkpoints
         if self.fused is not None:
             self.fused.pack_from(self._shared.ptr, base)      # straight out of the learner's memory
+        elif self.codes is not None:
+            self._quantize()
         torch.cuda.current_stream(self.device).synchronize()
         return True
 
@@ -191,6 +209,9 @@ class GpuActor:
         out = self.out[:n] if out is None else out
         if self.fused is not None:
             self.fused.infer(self.fused.infer_args(obs, out, n, self.action_scale), n)
+            return out
+        if self.codes is not None:
+            torch.mul(mlp3_int8(obs[:, : self.S], self.codes, "tanh"), self.action_scale, out=out[:, : self.A])
             return out
         (w1, b1, s1), (w2, b2, s2), (w3, b3, s3) = self._slot(0), self._slot(1), self._slot(2)
         H.gemm_group([H.gemm_desc(H.GEMM_NT, obs, obs.shape[1], w1, s1.ld, self.h1, self.ldh, n, self.Hd, self.S,
@@ -224,3 +245,5 @@ class GpuActor:
         self.view.load_state_dict(sd, strict)
         if self.fused is not None:
             self.fused.pack_from(self.flat.data_ptr())
+        elif self.codes is not None:
+            self._quantize()

@@ -111,6 +111,8 @@ EXTENSION_DEFAULTS: Dict[str, Any] = {
                                      # MFMA, fused row-local pipeline, tracks eager PyTorch to rounding) | "bf16"
                                      # (opt-in: the same pipeline with bf16 MFMA operands; fp32 master weights, Adam,
                                      # logits and loss)
+    "policy_precision": "fp32",      # agents that act on a GPU: "fp32" | "int8" (weights quantised per output channel, states and
+                                     # hidden activations per row; ops/int8.py).  Training stays as compute_dtype says
     "use_hip_graph": True,           # replay the whole update as one captured HIP graph
     "fused_learner": "auto",         # "auto": HIP kernels on cuda, torch ops on cpu; "torch": force eager torch;
                                      # "layers": the fp32 kernels with one launch per layer (any shape)
@@ -298,6 +300,7 @@ def finalize_config(raw: Dict[str, Any]) -> Dict[str, Any]:
     need(all(d >= 0 for d in cfg["rollout_devices"]), "rollout_devices must be GPU indices")
     need(cfg["critic_loss"] in ("bce", "ce"), "critic_loss must be 'bce' or 'ce'")
     need(cfg["compute_dtype"] in ("auto", "fp32", "bf16"), "compute_dtype must be 'auto', 'fp32' or 'bf16'")
+    need(cfg["policy_precision"] in ("fp32", "int8"), "policy_precision must be 'fp32' or 'int8'")
     need(cfg["replay_device"] in ("auto", "hbm", "host"), "replay_device must be auto|hbm|host")
     need(cfg["log_backend"] in ("tb", "jsonl", "both"), "log_backend must be tb|jsonl|both")
     if model == "d4pg":

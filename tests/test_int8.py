@@ -225,15 +225,25 @@ def _check_linear(y, q, scale, w, ws, b, act, dtype):
 
 SHAPES = [(1, 1, 1), (1, 3, 15), (2, 4, 16), (1, 400, 400), (3, 5, 17), (16, 16, 64), (17, 33, 65), (1, 50, 1000), (5, 17, 127),
           (31, 31, 129), (64, 51, 400), (65, 64, 256), (128, 128, 128), (129, 130, 131), (256, 400, 400), (300, 7, 2001),
-          (7, 300, 2001), (257, 513, 640), (500, 260, 1111), (2, 4096, 1024), (1030, 1025, 385), (40, 2050, 96),
-          # one shape at least for every tile size and row kernel, all with ragged edges
-          (3585, 3333, 300), (2300, 1700, 1300), (1793, 1665, 700), (700, 900, 5000), (150, 4000, 4100), (130, 4090, 1100), (1000, 1030, 1023),
+          (7, 300, 2001), (257, 513, 640), (500, 260, 1111), (2, 4096, 1024), (1030, 1025, 385), (40, 2050, 96)]
+#: one shape at least for every tile size and row kernel, all with ragged edges
+GPU_SHAPES = [(3585, 3333, 300), (2300, 1700, 1300), (1793, 1665, 700), (700, 900, 5000), (150, 4000, 4100), (130, 4090, 1100), (1000, 1030, 1023),
           (16, 12300, 200), (3, 12289, 70), (9, 3000, 4100), (30, 7000, 333), (31, 20000, 50), (60, 3100, 77), (900, 300, 1000), (17, 330, 128)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", GPU_SHAPES)
+def test_linear_int8_by_every_kernel(M, N, K):
+    _linear_case(M, N, K, "cuda")
 
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("M,N,K", SHAPES)
 def test_linear_int8(M, N, K, device):
+    _linear_case(M, N, K, device)
+
+
+def _linear_case(M, N, K, device):
     q, scale = _codes(M, K, device, seed=M + 3 * N + 7 * K)
     w, ws = _codes(N, K, device, seed=K)
     b = _randn(N, seed=4).to(device)
@@ -482,6 +492,52 @@ def test_on_another_stream_and_captured():
         torch.cuda.synchronize()
         got = [o.clone() for o in outs]
         assert all(torch.equal(a, c) for a, c in zip(got, chain()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S,A,Hd,E", [(24, 4, 400, 16), (111, 8, 1024, 300), (3, 1, 2400, 5)])
+def test_a_gpu_agent_acts_on_8_bit_codes(S, A, Hd, E):
+    """The agent's policy is ``mlp3_int8`` on codes of its parameters, whichever way these arrive, and stays near the
+    fp32 policy: three layers of codes are off by about 1 % of a layer's values each."""
+    import numpy as np
+
+    from d4pg_pytorch_amd.actors.gpu_actor import GpuActor
+    from d4pg_pytorch_amd.models.nets import ActorPolicy, init_net_
+    pol = ActorPolicy(S, A, Hd)
+    init_net_(pol.view, 0.05, _gen(3))
+    ga = GpuActor(S, A, Hd, max_batch=E, action_scale=1.5, precision="int8")
+    x = _randn(E, S, seed=4)
+    zero = ga.act(x.numpy())
+    assert zero.shape == (E, A) and not zero.any()                  # parameters of zeros
+    ga.load_flat(pol.flat.numpy())
+    got = ga.act(x.numpy())
+    layers = [(*ops.quantize_rows(w.cuda()), b.cuda()) for w, b in zip(pol.view.weights, pol.view.biases)]
+    assert np.array_equal(got, (1.5 * ops.mlp3_int8(x.cuda(), layers, "tanh")).cpu().numpy())
+    want = 1.5 * pol.act(x).numpy()
+    assert np.linalg.norm(got - want) <= 0.05 * np.linalg.norm(want)
+    init_net_(pol.view, 0.05, _gen(9))
+    ga.load_state_dict(pol.state_dict())
+    assert np.linalg.norm(ga.act(x.numpy()) - 1.5 * pol.act(x).numpy()) <= 0.05 * np.linalg.norm(want)
+    assert np.array_equal(ga.act(x[0].numpy())[0], ga.act(x.numpy())[0])
+    with pytest.raises(ValueError):
+        GpuActor(S, A, Hd, precision="int4")
+
+
+def test_the_agents_precision_is_a_config_key():
+    from d4pg_pytorch_amd.config import ConfigError, default_config
+    assert default_config(env="Pendulum-v0")["policy_precision"] == "fp32"
+    assert default_config(env="Pendulum-v0", policy_precision="int8")["policy_precision"] == "int8"
+    with pytest.raises(ConfigError):
+        default_config(env="Pendulum-v0", policy_precision="fp8")
+
+
+@pytest.mark.gpu
+def test_the_config_key_reaches_the_agent():
+    from d4pg_pytorch_amd.actors.agent import make_policy
+    from d4pg_pytorch_amd.config import default_config
+    cfg = default_config(env="Pendulum-v0", policy_precision="int8", dense_size=64)
+    assert make_policy(cfg, "cuda").precision == "int8" and make_policy(cfg, "cuda").launches_per_act == 2
+    assert make_policy(dict(cfg, policy_precision="fp32"), "cuda").precision == "fp32"
 
 
 def test_parameters_that_want_gradients_are_served_without():
