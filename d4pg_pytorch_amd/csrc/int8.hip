@@ -856,11 +856,9 @@ __device__ __forceinline__ bool mlp_move(MlpFeed<TPW>& f, const Mlp3Int8Args& a,
 }
 
 // Codes of row r, columns n .. n + 3 of one lane's values.
-__device__ __forceinline__ void mlp_codes(signed char* codes, int pitch, int r, int n, int N, const float (&v)[4], const RowCode& rc) {
-    unsigned b[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) b[i] = n + i < N ? code_bits(v[i], rc) & rc.keep : 0u;
-    *reinterpret_cast<unsigned*>(codes + r * pitch + n) = pack4(b[0], b[1], b[2], b[3]);
+__device__ __forceinline__ void mlp_codes(signed char* codes, int pitch, int r, int n, const float (&v)[4], const RowCode& rc) {
+    *reinterpret_cast<unsigned*>(codes + r * pitch + n) =
+        pack4(code_bits(v[0], rc), code_bits(v[1], rc), code_bits(v[2], rc), code_bits(v[3], rc)) & rc.keep;
 }
 
 // LDS of a workgroup: the waves' rings, their columns (64 scales and 64 biases each), codes, sums of narrow layers, tops.
@@ -986,18 +984,25 @@ __device__ __forceinline__ void mlp3_rows(const Mlp3Int8Args& a, signed char* co
         if (s.slices * NB < AHEAD) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         // Values of this wave: wide layers TPW x MT tiles; narrow ones the sums of all waves, dealt out again as units
         // (tile, 16 rows), of which a wave has at most one.
-        float v[TPW][MT][4];
+        float v[TPW][MT][4], sm[MT];
         unsigned m[MT] = {};
-        auto finish = [&](float (&y)[4], const i32x4 sum, int r, int n, int col, unsigned& most) {
-            Columns4 cc;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) cc.scale[e] = cols[col + e], cc.bias[e] = biased ? cols[64 + col + e] : 0.f;
-            values4(y, scaled4(sum, row_code(top_in[r]).scale), cc, biased, act);
+        for (int i = 0; i < MT; ++i) sm[i] = row_code(top_in[16 * (s.narrow ? ui : i) + c]).scale;
+        auto finish = [&](float (&y)[4], const i32x4 sum, float sr, int r, int n, int col, unsigned& most) {
+            Columns4 cc;
+            *reinterpret_cast<f32x4*>(cc.scale) = *reinterpret_cast<const f32x4*>(cols + col);
+            *reinterpret_cast<f32x4*>(cc.bias) = *reinterpret_cast<const f32x4*>(cols + 64 + col);
+            values4(y, scaled4(sum, sr), cc, biased, act);
             if (layer == 2) {
                 if (m0 + r < a.M && n < N) store_values4(a.out, (long long)(m0 + r) * a.ld_out + n, a.dtype, y, N - n);
             } else {
+                // beyond the layer's width the last column again (its scale and bias, some weight row's sum): no value
+                if (n + 4 > N) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) most = max(most, n + e < N ? abs_bits(y[e]) : 0u);
+                    for (int e = 0; e < 4; ++e) y[e] = n + e < N ? y[e] : 0.f;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) most = max(most, abs_bits(y[e]));
             }
         };
         if (s.narrow) {
@@ -1014,14 +1019,14 @@ __device__ __forceinline__ void mlp3_rows(const Mlp3Int8Args& a, signed char* co
                 i32x4 sum;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sum[e] = from[e * 64], from[e * 64] = 0;   // zeros for the next layer that needs them
-                finish(v[0][0], sum, 16 * ui + c, 16 * ut + 4 * g, 4 * g, m[0]);
+                finish(v[0][0], sum, sm[0], 16 * ui + c, 16 * ut + 4 * g, 4 * g, m[0]);
             }
         } else {
 #pragma unroll
             for (int j = 0; j < TPW; ++j)
                 if (j < s.count)
 #pragma unroll
-                    for (int i = 0; i < MT; ++i) finish(v[j][i], acc[j][i], 16 * i + c, 16 * (s.tile0 + MLP_WAVES * j) + 4 * g, 16 * j + 4 * g, m[i]);
+                    for (int i = 0; i < MT; ++i) finish(v[j][i], acc[j][i], sm[i], 16 * i + c, 16 * (s.tile0 + MLP_WAVES * j) + 4 * g, 16 * j + 4 * g, m[i]);
         }
         if (layer == 2) break;
 #pragma unroll
@@ -1040,14 +1045,14 @@ __device__ __forceinline__ void mlp3_rows(const Mlp3Int8Args& a, signed char* co
             if (n >= 16 * s.tiles) *reinterpret_cast<i32x4*>(codes + (threadIdx.x >> 2) * pitch + n) = i32x4{0, 0, 0, 0};
         }
         if (s.narrow) {
-            if (ut < s.tiles) mlp_codes(codes, pitch, 16 * ui + c, 16 * ut + 4 * g, N, v[0][0], row_code(top_out[16 * ui + c]));
+            if (ut < s.tiles) mlp_codes(codes, pitch, 16 * ui + c, 16 * ut + 4 * g, v[0][0], row_code(top_out[16 * ui + c]));
         } else {
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 const RowCode rc = row_code(top_out[16 * i + c]);
 #pragma unroll
                 for (int j = 0; j < TPW; ++j)
-                    if (j < s.count) mlp_codes(codes, pitch, 16 * i + c, 16 * (s.tile0 + MLP_WAVES * j) + 4 * g, N, v[j][i], rc);
+                    if (j < s.count) mlp_codes(codes, pitch, 16 * i + c, 16 * (s.tile0 + MLP_WAVES * j) + 4 * g, v[j][i], rc);
             }
         }
         lds_barrier();
