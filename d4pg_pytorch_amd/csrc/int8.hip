@@ -320,12 +320,27 @@ __global__ __launch_bounds__(1024) void quant_long_rows_kernel(const QuantRowsAr
     if (threadIdx.x == 0) a.scale[row] = code.scale;
 }
 
+// A launch holds fewer than 2^32 threads: more rows than that are several launches.
+template <typename F>
+static void launch_row_ranges(QuantRowsArgs a, long long element, int block, int rows_per_block, F launch) {
+    const long long most = (0xffffffffll / block) * rows_per_block, M = a.M;
+    for (long long done = 0; done < M; done += most) {
+        QuantRowsArgs part = a;
+        part.M = M - done < most ? M - done : most;
+        part.x = (const char*)a.x + done * a.ld_x * element;
+        if (a.residual != nullptr) part.residual = (const char*)a.residual + done * a.ld_r * element;
+        if (a.h != nullptr) part.h = (char*)a.h + done * a.ld_h * element;
+        part.q = a.q + done * a.ld_q, part.scale = a.scale + done;
+        launch(part, dim3((unsigned)((part.M + rows_per_block - 1) / rows_per_block)));
+    }
+}
 template <typename T, int G, int V>
 static void launch_rows(const QuantRowsArgs& a, hipStream_t stream) {
-    constexpr int BLOCK = G < 256 ? 256 : G, RPB = BLOCK / G;
-    const dim3 grid((unsigned)((a.M + RPB - 1) / RPB)), block(BLOCK);
-    if (a.norm) hipLaunchKernelGGL((quant_rows_kernel<T, G, V, true>), grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((quant_rows_kernel<T, G, V, false>), grid, block, 0, stream, a);
+    constexpr int BLOCK = G < 256 ? 256 : G;
+    launch_row_ranges(a, sizeof(T), BLOCK, BLOCK / G, [&](const QuantRowsArgs& part, dim3 grid) {
+        if (a.norm) hipLaunchKernelGGL((quant_rows_kernel<T, G, V, true>), grid, dim3(BLOCK), 0, stream, part);
+        else hipLaunchKernelGGL((quant_rows_kernel<T, G, V, false>), grid, dim3(BLOCK), 0, stream, part);
+    });
 }
 template <typename T>
 static void launch_rows_of(const QuantRowsArgs& a, hipStream_t stream) {
@@ -338,11 +353,11 @@ static void launch_rows_of(const QuantRowsArgs& a, hipStream_t stream) {
     else if (c <= 1024) launch_rows<T, 256, 4>(a, stream);
     else if (c <= 2048) launch_rows<T, 256, 8>(a, stream);
     else if (c <= 4096) launch_rows<T, 1024, 4>(a, stream);
-    else {
-        const dim3 grid((unsigned)a.M), block(1024);
-        if (a.norm) hipLaunchKernelGGL((quant_long_rows_kernel<T, true>), grid, block, 0, stream, a);
-        else hipLaunchKernelGGL((quant_long_rows_kernel<T, false>), grid, block, 0, stream, a);
-    }
+    else
+        launch_row_ranges(a, sizeof(T), 1024, 1, [&](const QuantRowsArgs& part, dim3 grid) {
+            if (a.norm) hipLaunchKernelGGL((quant_long_rows_kernel<T, true>), grid, dim3(1024), 0, stream, part);
+            else hipLaunchKernelGGL((quant_long_rows_kernel<T, false>), grid, dim3(1024), 0, stream, part);
+        });
 }
 
 D4PG_API int d4pg_quant_rows(const QuantRowsArgs* a, hipStream_t stream) {
@@ -389,11 +404,18 @@ D4PG_API int d4pg_dequant_rows(DequantRowsArgs* a, hipStream_t stream) {
     a->tpr_log = 0;
     while (a->tpr_log < 8 && (8ll << a->tpr_log) < a->K) ++a->tpr_log;
     const int rpb = 256 >> a->tpr_log;
-    const dim3 grid((unsigned)((a->M + rpb - 1) / rpb)), block(256);
-    if (a->dtype == F_FP32) hipLaunchKernelGGL(dequant_rows_kernel<float>, grid, block, 0, stream, *a);
-    else if (a->dtype == F_BF16) hipLaunchKernelGGL(dequant_rows_kernel<__bf16>, grid, block, 0, stream, *a);
-    else if (a->dtype == F_FP16) hipLaunchKernelGGL(dequant_rows_kernel<_Float16>, grid, block, 0, stream, *a);
-    else return -6;
+    const long long most = (0xffffffffll / 256) * rpb;
+    const int bytes = a->dtype == F_FP32 ? 4 : 2;
+    if (a->dtype < F_FP32 || a->dtype > F_FP16) return -6;
+    for (long long done = 0; done < a->M; done += most) {       // fewer than 2^32 threads a launch
+        DequantRowsArgs part = *a;
+        part.M = a->M - done < most ? a->M - done : most;
+        part.q = a->q + done * a->ld_q, part.scale = a->scale + done, part.out = (char*)a->out + done * a->K * bytes;
+        const dim3 grid((unsigned)((part.M + rpb - 1) / rpb)), block(256);
+        if (a->dtype == F_FP32) hipLaunchKernelGGL(dequant_rows_kernel<float>, grid, block, 0, stream, part);
+        else if (a->dtype == F_BF16) hipLaunchKernelGGL(dequant_rows_kernel<__bf16>, grid, block, 0, stream, part);
+        else hipLaunchKernelGGL(dequant_rows_kernel<_Float16>, grid, block, 0, stream, part);
+    }
     return (int)hipGetLastError();
 }
 
@@ -459,6 +481,8 @@ __device__ __forceinline__ void finish4(const LinearInt8Args& a, int m, int n, c
     values4(v, scaled, c, a.bias != nullptr, a.act);
     store_values4(a.out, (long long)m * a.ld_out + n, a.dtype, v, a.N - n);
 }
+
+enum { TOO_MANY = -7 };        // threads for one launch: the caller halves the rows
 
 // All ones in the bytes k .. k + 15 that lie below K.
 __device__ __forceinline__ i32x4 below(int k, int K) {
@@ -546,6 +570,7 @@ __global__ __launch_bounds__(64 * WAVES) void linear_int8_rows_kernel(const Line
 template <int MT, int NT, int WAVES, int U>
 static int launch_linear_rows(const LinearInt8Args& a, hipStream_t stream) {
     const long long tiles = (long long)((a.M + 16 * MT - 1) / (16 * MT)) * ((a.N + 16 * NT - 1) / (16 * NT));
+    if (tiles * (64 * WAVES) > 0xffffffffll) return TOO_MANY;
     hipLaunchKernelGGL((linear_int8_rows_kernel<MT, NT, WAVES, U>), dim3((unsigned)tiles), dim3(64 * WAVES), 0, stream, a);
     return (int)hipGetLastError();
 }
@@ -709,7 +734,7 @@ static int launch_linear_tiles(const LinearInt8Args& a, hipStream_t stream) {
     constexpr int BM = 32 * MI * WM, BN = 32 * NI * WN, TILES = S * (BM + BN) * 128, STAGE = WM * WN * (32 * (32 * NI + 4) * 4 + (KW == 2 ? NI * MI * 4096 : 0));
     constexpr int LDS = TILES > STAGE ? TILES : STAGE;
     const long long tiles = (long long)((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN);
-    if (tiles > 0x7fffffffll) return -7;
+    if (tiles * (64 * WM * WN * KW) > 0xffffffffll) return TOO_MANY;
     hipLaunchKernelGGL((linear_int8_tiles_kernel<MI, NI, WM, WN, KW, S>), dim3((unsigned)tiles), dim3(64 * WM * WN * KW), LDS, stream, a);
     return (int)hipGetLastError();
 }
@@ -755,16 +780,29 @@ static int launch_linear(const LinearInt8Args& a, long long kp, hipStream_t stre
     return launch_linear_rows<4, 2, 8, 2>(a, stream);
 }
 
+static int linear_rows_of(const LinearInt8Args& a, long long kp, hipStream_t stream) {
+    int rc = a.M > 1 << 30 ? (int)TOO_MANY : launch_linear(a, kp, stream);      // row numbers past M stay 32-bit
+    if (rc != TOO_MANY || a.M <= 256) return rc;
+    LinearInt8Args part = a;
+    part.M = (a.M / 2 + 255) & ~255;
+    rc = linear_rows_of(part, kp, stream);
+    if (rc != 0) return rc;
+    part = a;
+    const long long done = (a.M / 2 + 255) & ~255;
+    part.M -= (int)done, part.q += done * a.ld_q, part.scale += done;
+    part.out = (char*)a.out + done * a.ld_out * (a.dtype == F_FP32 ? 4 : 2);
+    return linear_rows_of(part, kp, stream);
+}
+
 D4PG_API int d4pg_linear_int8(const LinearInt8Args* a, hipStream_t stream) {
-    if (a->M < 1 || a->N < 1 || a->K < 1 || a->K >= 131072) return -1;
+    if (a->M < 1 || a->N < 1 || a->N > 1 << 30 || a->K < 1 || a->K >= 131072) return -1;
     if (a->q == nullptr || a->w == nullptr || a->scale == nullptr || a->wscale == nullptr || a->out == nullptr) return -2;
     const long long kp = (a->K + 15) & ~15;
     if (((a->M > 1 ? a->ld_q : 16) & 15) || ((a->N > 1 ? a->ld_w : 16) & 15)) return -3;
     if ((a->M > 1 && a->ld_q < kp) || (a->N > 1 && a->ld_w < kp) || (a->M > 1 && a->ld_out < a->N)) return -4;
     if (((uintptr_t)a->q | (uintptr_t)a->w) & 15) return -5;
     if (a->dtype < F_FP32 || a->dtype > F_FP16 || a->act < ACT_NONE || a->act > ACT_TANH) return -6;
-    if ((long long)((a->M + 15) / 16) * ((a->N + 15) / 16) > 0x7fffffffll) return -7;
-    return launch_linear(*a, kp, stream);
+    return linear_rows_of(*a, kp, stream);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -1094,9 +1132,9 @@ D4PG_API int d4pg_mlp3_int8(Mlp3Int8Args* a, hipStream_t stream) {
         if (tiles > wide_out) wide_out = tiles;
         if (tiles <= MLP_WAVES / 2 && tiles > few) few = tiles;
     }
-    if (widest > 2048 || wide_out > 64) return 1;
+    if (widest > 2048 || wide_out > 64 || a->M > 1 << 25) return 1;       // (2^25 rows: 2^31 threads)
     a->pitch = ((widest + 63) & ~63) + 16;
-    const bool two = a->pad_ ? a->pad_ == 2 : a->M > 4096;        // 32 rows a workgroup
+    const bool two = a->M > 4096;                // 32 rows a workgroup, so that one round of workgroups holds them longer
     if (wide_out <= 16) return two ? launch_mlp3<1, 2>(*a, few, stream) : launch_mlp3<1, 1>(*a, few, stream);
     if (wide_out <= 32) return two ? launch_mlp3<2, 2>(*a, few, stream) : launch_mlp3<2, 1>(*a, few, stream);
     if (two) return launch_mlp3<4, 2>(*a, few, stream);

@@ -52,6 +52,5 @@ struct Mlp3Int8Args {
     long long ld_x, ld_out, ld_w[3];
     int M, width[4];
     int xdtype, dtype, act;        // F_* of x and out; ACT_* of the last layer (the others: ReLU)
-    int pad_;
     int pitch, split;              // bytes of a row of codes in LDS, words of the split layers' sums (set by the host entry)
 };

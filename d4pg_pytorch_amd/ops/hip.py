@@ -396,7 +396,7 @@ class Mlp3Int8Args(C.Structure):
     _fields_ = [("x", vp), ("out", vp), ("w", vp * 3), ("wscale", vp * 3), ("bias", vp * 3),
                 ("ld_x", C.c_longlong), ("ld_out", C.c_longlong), ("ld_w", C.c_longlong * 3),
                 ("M", C.c_int), ("width", C.c_int * 4), ("xdtype", C.c_int), ("dtype", C.c_int), ("act", C.c_int),
-                ("pad_", C.c_int), ("pitch", C.c_int), ("split", C.c_int)]
+                ("pitch", C.c_int), ("split", C.c_int)]
 
 
 class DevStateMirror(C.Structure):

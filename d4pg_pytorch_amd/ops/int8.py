@@ -236,6 +236,8 @@ def _layer(device: torch.device, K: int, weight: torch.Tensor, weight_scale: tor
         raise ValueError(f"weight has shape {tuple(weight.shape)}, expected (out, {K})")
     if K > MAX_K:
         raise ValueError(f"{K} columns: sums of more than {MAX_K} products can leave 32 bits")
+    if weight.shape[0] > 1 << 30:
+        raise ValueError(f"{weight.shape[0]} outputs: at most 2^30 are supported")
     _on(device, "weight", weight)
     outs = weight.shape[:1]
     return _vector(device, "weight_scale", weight_scale, outs), None if bias is None else _vector(device, "bias", bias, outs)

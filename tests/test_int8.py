@@ -466,6 +466,22 @@ def test_a_residual_block_of_them(device):
 
 
 @pytest.mark.gpu
+def test_more_rows_than_one_launch_holds():
+    """64 threads a row: 2^26 rows are 2^32 threads, which is one too many for a launch; offsets pass 32 bits too."""
+    M = (1 << 26) + 70
+    x = torch.arange(M, device="cuda", dtype=torch.float32).remainder_(251.0).sub_(125.0)[:, None]
+    q, scale = ops.quantize_rows(x)
+    assert torch.equal(q, (x.sign() * 127).to(torch.int8))
+    assert torch.all((scale.double() - x[:, 0].abs().double() / 127).abs() <= scale.double() * U)
+    back = ops.dequantize_rows(q, scale, torch.bfloat16)
+    assert torch.equal(back, (q.float() * scale[:, None]).bfloat16())
+    del back
+    w, ws = _codes(1, 1, "cuda", 3)
+    y = ops.linear_int8(q, scale, w, ws)
+    assert torch.equal(y, (q.float() * w.float()) * scale[:, None] * ws)
+
+
+@pytest.mark.gpu
 def test_on_another_stream_and_captured():
     x = _randn(65, 200, seed=1).cuda()
     r = _randn(65, 200, seed=2).cuda()
@@ -565,7 +581,7 @@ def test_the_library_refuses_what_its_kernels_cannot_read():
             setattr(a, k, v)
         return lib.d4pg_linear_int8(C.byref(a), None)
 
-    for kw in (dict(M=0), dict(N=0), dict(K=0), dict(K=131072), dict(q=None), dict(w=None), dict(scale=None), dict(wscale=None),
+    for kw in (dict(M=0), dict(N=0), dict(N=(1 << 30) + 1), dict(K=0), dict(K=131072), dict(q=None), dict(w=None), dict(scale=None), dict(wscale=None),
                dict(out=None), dict(ld_q=40), dict(ld_w=24), dict(ld_q=16), dict(ld_w=16), dict(ld_out=3), dict(q=4104), dict(w=8193),
                dict(dtype=3), dict(dtype=-1), dict(act=3), dict(act=-1)):
         assert product(**kw) < 0, kw
