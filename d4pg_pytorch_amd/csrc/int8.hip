@@ -45,20 +45,32 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
     __builtin_memcpy(p, &r, sizeof(r));
 }
 
-__device__ __forceinline__ unsigned wave_umax(unsigned v) {
+__device__ __forceinline__ unsigned row16_umax(unsigned v) {       // over 16 neighbouring lanes
     v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xb1, 0xf, 0xf, false));
     v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4e, 0xf, 0xf, false));
     v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false));
     v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false));
+    return v;
+}
+__device__ __forceinline__ float row16_sum(float v) {
+    v += dpp_mov<0xb1>(v);
+    v += dpp_mov<0x4e>(v);
+    v += dpp_mov<0x124>(v);
+    v += dpp_mov<0x128>(v);
+    return v;
+}
+__device__ __forceinline__ unsigned wave_umax(unsigned v) {
+    v = row16_umax(v);
     const unsigned a = __builtin_amdgcn_readlane((int)v, 0), b = __builtin_amdgcn_readlane((int)v, 16);
     const unsigned c = __builtin_amdgcn_readlane((int)v, 32), d = __builtin_amdgcn_readlane((int)v, 48);
     return max(max(a, b), max(c, d));
 }
 
-// Sum / maximum over the G threads that share a row.  G = 64: one wave, no LDS.  `red` holds 32 words; two of them
-// alternate between calls so that one barrier a call is enough.
+// Sum / maximum over the G threads that share a row.  G = 16 and 64: lanes of one wave, no LDS.  `red` holds a word a wave,
+// and every call of a kernel has words of its own, so that one barrier a call is enough.
 template <int G>
 __device__ __forceinline__ float group_sum(float v, unsigned* red) {
+    if constexpr (G == 16) return row16_sum(v);
     v = wave_sum(v);
     if constexpr (G == 64) return v;
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = __builtin_bit_cast(unsigned, v);
@@ -70,6 +82,7 @@ __device__ __forceinline__ float group_sum(float v, unsigned* red) {
 }
 template <int G>
 __device__ __forceinline__ unsigned group_umax(unsigned v, unsigned* red) {
+    if constexpr (G == 16) return row16_umax(v);
     v = wave_umax(v);
     if constexpr (G == 64) return v;
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
@@ -151,14 +164,17 @@ __device__ __forceinline__ void scale8(float (&y)[8], const void* weight, long l
     for (int i = 0; i < 8; ++i) y[i] *= (float)w.e[i];
 }
 
+// What bounds it is memory: quantising 8192 x 8192 bf16 takes 32.5 us (6.2 TB/s read and written), 2000 x 16384 fp32 25.7 us
+// (6.4), the norm with a residual of 4096 x 4096 bf16 22 us (5.3), of 16384 x 8192 175 us (5.4); a copy of 1 GiB runs at 5.2.
+// Rows of odd length (16384 x 1111 bf16, loads across cache lines) get 3.3 TB/s.
 // A row stays in the registers of its G threads from the load to the codes: one read, one write, whatever is computed
 // between.  Thread t holds the 8-element chunks t, t + G, ... (V of them).
 template <typename T, int G, int V, bool NORM>
 __global__ __launch_bounds__(G < 256 ? 256 : G) void quant_rows_kernel(const QuantRowsArgs a) {
     constexpr int BLOCK = G < 256 ? 256 : G;
-    __shared__ unsigned red[4][G > 64 ? G / 64 : 1];
+    __shared__ unsigned red[4][G > 64 ? G / 64 : 1];       // one line a reduction
     const long long row = (long long)blockIdx.x * (BLOCK / G) + threadIdx.x / G;
-    if (row >= a.M) return;                      // whole waves (G = 64) only: no barrier is skipped
+    if (row >= a.M) return;                      // whole groups of 16 or 64 lanes only: no barrier is skipped
     const int t = threadIdx.x % G;
     const int K = (int)a.K, full = K >> 3, rem = K & 7, chunks = (int)(a.ld_q >> 3);
     const T* const x = reinterpret_cast<const T*>(a.x) + row * a.ld_x;
@@ -271,7 +287,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void quant_rows_kernel(const Qua
     if (t == 0) a.scale[row] = code.scale;
 }
 
-// Rows too long for the registers of 1024 threads: the row is read again for each of the three steps.
+// Rows too long for the registers of 1024 threads: the row is read again for each of the steps (it fits the L2 once).
 template <typename T, bool NORM>
 __global__ __launch_bounds__(1024) void quant_long_rows_kernel(const QuantRowsArgs a) {
     constexpr int G = 1024;
@@ -281,27 +297,55 @@ __global__ __launch_bounds__(1024) void quant_long_rows_kernel(const QuantRowsAr
     const T* const r = reinterpret_cast<const T*>(a.residual) + row * a.ld_r;
     T* const h = reinterpret_cast<T*>(a.h) + row * a.ld_h;
     const bool add = NORM && a.residual != nullptr;
-    const long long K = a.K;
-    auto value = [&](long long k) { return (float)x[k] + (add ? (float)r[k] : 0.f); };
-    float pre = 1.f, rs = 1.f;
+    const int K = (int)a.K, full = K >> 3, rem = K & 7, chunks = (int)(a.ld_q >> 3);
+    // chunk c of the sum x + residual, zeros beyond the row
+    auto sums8 = [&](int c, float (&y)[8]) {
+        if (c < full) {
+            const Raw8<T> rx = load8(x + 8ll * c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = (float)rx.e[i];
+            if (add) {
+                const Raw8<T> rr = load8(r + 8ll * c);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] += (float)rr.e[i];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = c == full && i < rem ? (float)x[8ll * c + i] + (add ? (float)r[8ll * c + i] : 0.f) : 0.f;
+        }
+    };
+    float pre = 1.f, rs = 1.f, y[8];
     if (NORM) {
         float ss = 0.f;
-        for (long long k = threadIdx.x; k < K; k += G) {
-            const float v = value(k);
-            ss += v * v;
-            if (a.h != nullptr) h[k] = (T)v;
+        for (int c = threadIdx.x; c < chunks; c += G) {
+            sums8(c, y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss += y[i] * y[i];
+            if (a.h != nullptr) {
+                if (c < full) store8(h + 8ll * c, y);
+                else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (c == full && i < rem) h[8ll * c + i] = (T)y[i];
+                }
+            }
         }
         ss = group_sum<G>(ss, red[0]);
         float eps = a.eps;
         if (!norm_is_plain(ss, (float)K, eps)) {
             unsigned top = 0;
-            for (long long k = threadIdx.x; k < K; k += G) top = max(top, abs_bits(value(k)));
+            for (int c = threadIdx.x; c < chunks; c += G) {
+                sums8(c, y);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = max(top, abs_bits(y[i]));
+            }
             top = group_umax<G>(top, red[1]);
             pre = norm_lift(top, eps);
             ss = 0.f;
-            for (long long k = threadIdx.x; k < K; k += G) {
-                const float v = value(k) * pre;
-                ss += v * v;
+            for (int c = threadIdx.x; c < chunks; c += G) {
+                sums8(c, y);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) ss += (y[i] * pre) * (y[i] * pre);
             }
             ss = group_sum<G>(ss, red[2]);
             eps = eps * pre * pre;
@@ -310,13 +354,36 @@ __global__ __launch_bounds__(1024) void quant_long_rows_kernel(const QuantRowsAr
         }
         rs = 1.f / sqrtf(ss / (float)K + eps);
     }
-    auto out = [&](long long k) { return NORM ? (value(k) * pre) * rs * weight1(a, k) : value(k); };
+    auto values8 = [&](int c) {
+        sums8(c, y);
+        if (NORM) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = (y[i] * pre) * rs;
+            if (a.wdtype != F_NONE) {
+                if (c < full) {
+                    if (a.wdtype == F_FP32) scale8<float>(y, a.weight, 8ll * c);
+                    else if (a.wdtype == F_BF16) scale8<__bf16>(y, a.weight, 8ll * c);
+                    else scale8<_Float16>(y, a.weight, 8ll * c);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (c == full && i < rem) y[i] *= weight1(a, 8ll * c + i);
+                }
+            }
+        }
+    };
     unsigned top = 0;
-    for (long long k = threadIdx.x; k < K; k += G) top = max(top, abs_bits(out(k)));
+    for (int c = threadIdx.x; c < chunks; c += G) {
+        values8(c);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, abs_bits(y[i]));
+    }
     const RowCode code = row_code(group_umax<G>(top, red[3]));
     signed char* const q = a.q + row * a.ld_q;
-    for (long long k = threadIdx.x; k < a.ld_q; k += G)
-        q[k] = k < K ? (signed char)(code_bits(out(k), code) & code.keep) : 0;
+    for (int c = threadIdx.x; c < chunks; c += G) {
+        values8(c);
+        store_codes8(q + 8ll * c, y, code);
+    }
     if (threadIdx.x == 0) a.scale[row] = code.scale;
 }
 
@@ -344,12 +411,18 @@ static void launch_rows(const QuantRowsArgs& a, hipStream_t stream) {
 }
 template <typename T>
 static void launch_rows_of(const QuantRowsArgs& a, hipStream_t stream) {
-    // chunks of 8 a row needs: as few threads as hold it in at most 4 (8 from 8192 columns) chunks each
+    // c: chunks of 8 a row needs.  Short rows share a wave, long ones take as few threads as hold them in 4 chunks each (8 from
+    // 8192 columns on); where the rows are fewer than the CUs, 1024 threads answer sooner than 256.  Measured: 65536 x 100 fp32
+    // 7.1 us, 18.5 with a wave
+    // a row; 1 x 16384 bf16 with a residual 5.0 us, 8.8 with 256 threads.
     const long long c = a.ld_q >> 3;
-    if (c <= 64) launch_rows<T, 64, 1>(a, stream);
+    if (c <= 16) launch_rows<T, 16, 1>(a, stream);
+    else if (c <= 32) launch_rows<T, 16, 2>(a, stream);
+    else if (c <= 64) launch_rows<T, 64, 1>(a, stream);
     else if (c <= 128) launch_rows<T, 64, 2>(a, stream);
     else if (c <= 256) launch_rows<T, 64, 4>(a, stream);
     else if (c <= 512) launch_rows<T, 256, 2>(a, stream);
+    else if (c <= 2048 && a.M <= 256) launch_rows<T, 1024, 2>(a, stream);
     else if (c <= 1024) launch_rows<T, 256, 4>(a, stream);
     else if (c <= 2048) launch_rows<T, 256, 8>(a, stream);
     else if (c <= 4096) launch_rows<T, 1024, 4>(a, stream);
@@ -377,6 +450,7 @@ D4PG_API int d4pg_quant_rows(const QuantRowsArgs* a, hipStream_t stream) {
 // codes -> floating rows
 // ---------------------------------------------------------------------------------------------------------------
 
+// 8192 x 8192 to bf16: 30.7 us (6.6 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void dequant_rows_kernel(const DequantRowsArgs a) {
     const int tpr = 1 << a.tpr_log;
@@ -385,7 +459,7 @@ __global__ __launch_bounds__(256) void dequant_rows_kernel(const DequantRowsArgs
     const float s = a.scale[row];
     const signed char* const q = a.q + row * a.ld_q;
     T* const out = reinterpret_cast<T*>(a.out) + row * a.K;
-    for (long long k = 8ll * (threadIdx.x & (tpr - 1)); k < a.K; k += 8ll * tpr) {
+    for (long long k = 8ll * ((threadIdx.x & (tpr - 1)) + tpr * blockIdx.y); k < a.K; k += 8ll * tpr * gridDim.y) {
         if (k + 8 <= a.K) {
             const Raw8<signed char> c = load8(q + k);
             float v[8];
@@ -411,7 +485,9 @@ D4PG_API int d4pg_dequant_rows(DequantRowsArgs* a, hipStream_t stream) {
         DequantRowsArgs part = *a;
         part.M = a->M - done < most ? a->M - done : most;
         part.q = a->q + done * a->ld_q, part.scale = a->scale + done, part.out = (char*)a->out + done * a->K * bytes;
-        const dim3 grid((unsigned)((part.M + rpb - 1) / rpb)), block(256);
+        // few long rows: several workgroups each
+        const long long blocks = (part.M + rpb - 1) / rpb, pieces = (a->K + 2047) / 2048, spread = 1024 / blocks + 1;
+        const dim3 grid((unsigned)blocks, (unsigned)(spread < pieces ? spread : pieces)), block(256);
         if (a->dtype == F_FP32) hipLaunchKernelGGL(dequant_rows_kernel<float>, grid, block, 0, stream, part);
         else if (a->dtype == F_BF16) hipLaunchKernelGGL(dequant_rows_kernel<__bf16>, grid, block, 0, stream, part);
         else hipLaunchKernelGGL(dequant_rows_kernel<_Float16>, grid, block, 0, stream, part);
@@ -838,6 +914,12 @@ __device__ __forceinline__ float load_any(const void* p, int dtype, long long i)
 __device__ __forceinline__ void lds_barrier() {          // LDS is settled for the workgroup; moves stay on their way
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
+//
+// Measured (GPU time, us; the layers as launches of their own behind the /): 24-400-400-4 on one state 10.2 / 12.5, on 4096
+// states 12.7 / 30, on 8192 15.5 / 41; 111-1024-1024-8 on one state 18.6 / 13.8 (plus 22 of host time), on 4096 27.9 / 43, on
+// 8192 35.7 / 53.  At 4096 states of the latter 256 workgroups read 1.2 MB of weights each: 300 MB at the 18 TB/s that moves
+// alone reach would be 16 us.  At one state the chain of phases is what is left (clock stamps of a 400-wide network, cycles:
+// descriptors 2000, input 2400, layers 1200 + 4200 + 800, results and codes 1500 - 2500 each).
 struct MlpShare {                  // a wave's part of a layer: tiles tile0, tile0 + 16, ...; units of 64 k from k0, k_unit apart
     int K, N, tiles, count, tile0, k0, k_unit, slices;
     bool narrow;

@@ -152,7 +152,8 @@ def _norm64(x, weight, residual, eps):
                                            (5, 111, False, "same"), (4, 400, True, "same"), (2, 513, True, None),
                                            (3, 1111, False, "fp32"), (1, 2048, True, "same"), (2, 4096, True, "same"),
                                            (2, 4103, True, "fp32"), (2, 8192, False, "same"), (2, 16384, True, "same"),
-                                           (1, 20001, True, "same")])
+                                           (1, 20001, True, "same"), (33, 128, True, "fp32"), (19, 129, True, None), (300, 250, True, "same"),
+                                           (257, 5003, True, "same"), (300, 9001, False, "fp32"), (2, 33001, True, "fp32"), (2, 40008, True, None)])
 def test_add_rms_norm_int8(M, K, add, wtype, dtype, device):
     x = _randn(M, K, seed=K).to(dtype).to(device)
     r = (3 * _randn(M, K, seed=K + 1)).to(dtype).to(device) if add else None
