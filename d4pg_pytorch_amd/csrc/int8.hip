@@ -1018,12 +1018,17 @@ __device__ __forceinline__ void mlp3_rows(const Mlp3Int8Args& a, signed char* co
                                              (__attribute__((address_space(3))) void*)(cols + 64), 4, 0, 0);
     };
     const int S = a.width[0];
-    float held[MT][HELD];                        // first on their way: everything waits for the input
+    unsigned held[MT][HELD];                     // as bits, first on their way: everything waits for the input
+    auto hold = [&](auto bits) {                 // one branch for all of them: a branch each would wait for each
+        using B = decltype(bits);
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int p = 0; p < HELD; ++p)
-            held[i][p] = load_any(a.x, a.xdtype, (long long)min(m0 + wave + MLP_WAVES * i, a.M - 1) * a.ld_x + min(lane + 64 * p, S - 1));
+            for (int p = 0; p < HELD; ++p)
+                held[i][p] = reinterpret_cast<const B*>(a.x)[(long long)min(m0 + wave + MLP_WAVES * i, a.M - 1) * a.ld_x + min(lane + 64 * p, S - 1)];
+    };
+    if (a.xdtype == F_FP32) hold(0u);
+    else hold((unsigned short)0);
     MlpFeed<TPW> feed;
     feed.layer = 0, feed.slot = 0;
     mlp_open<TPW>(feed, a, wave, lane);
@@ -1038,8 +1043,14 @@ __device__ __forceinline__ void mlp3_rows(const Mlp3Int8Args& a, signed char* co
         const int r = wave + MLP_WAVES * i;
         const long long row = (long long)min(m0 + r, a.M - 1) * a.ld_x;
         unsigned t = 0;
+        float x[HELD];
 #pragma unroll
-        for (int p = 0; p < HELD; ++p) t = max(t, abs_bits(held[i][p]));     // beyond S: the last element again
+        for (int p = 0; p < HELD; ++p) {
+            x[p] = a.xdtype == F_FP32 ? __builtin_bit_cast(float, held[i][p])
+                 : a.xdtype == F_BF16 ? __builtin_bit_cast(float, held[i][p] << 16)
+                                      : (float)__builtin_bit_cast(_Float16, (unsigned short)held[i][p]);
+            t = max(t, abs_bits(x[p]));          // beyond S: the last element again
+        }
         for (int k = lane + 64 * HELD; k < S; k += 64) t = max(t, abs_bits(load_any(a.x, a.xdtype, row + k)));
         t = wave_umax(t);
         if (lane == 0) top[r] = t;
@@ -1047,7 +1058,7 @@ __device__ __forceinline__ void mlp3_rows(const Mlp3Int8Args& a, signed char* co
 #pragma unroll
         for (int p = 0; p < HELD; ++p) {
             const int k = lane + 64 * p;
-            if (k < padded) codes[r * pitch + k] = k < S ? (signed char)(code_bits(held[i][p], rc) & rc.keep) : 0;
+            if (k < padded) codes[r * pitch + k] = k < S ? (signed char)(code_bits(x[p], rc) & rc.keep) : 0;
         }
         for (int k = lane + 64 * HELD; k < padded; k += 64)
             codes[r * pitch + k] = k < S ? (signed char)(code_bits(load_any(a.x, a.xdtype, row + k), rc) & rc.keep) : 0;
