@@ -158,7 +158,10 @@ class GpuActor:
         elif self.fused is None:         # per-layer path: two hidden activation buffers
             self.h1 = torch.zeros(self.E, ldh, device=self.device)
             self.h2 = torch.zeros(self.E, ldh, device=self.device)
-        self.launches_per_act = 1 if self.fused is not None else (2 if precision == "int8" else 3)
+        if precision == "int8":        # the network (a launch a step beyond 1024 columns) and the way into the caller's actions
+            self.launches_per_act = 2 if max(state_dim, hidden) <= 1024 else 7
+        else:
+            self.launches_per_act = 1 if self.fused is not None else 3
         self._shared = None
         self._shared_half = 0
 

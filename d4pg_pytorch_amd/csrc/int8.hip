@@ -858,20 +858,21 @@ static int launch_linear(const LinearInt8Args& a, long long kp, hipStream_t stre
 
 static int linear_rows_of(const LinearInt8Args& a, long long kp, hipStream_t stream) {
     int rc = a.M > 1 << 30 ? (int)TOO_MANY : launch_linear(a, kp, stream);      // row numbers past M stay 32-bit
-    if (rc != TOO_MANY || a.M <= 256) return rc;
+    if (rc != TOO_MANY || a.M <= 16) return rc;
+    const int whole = a.M > 512 ? 255 : 15;
+    const long long done = (a.M / 2 + whole) & ~whole;
     LinearInt8Args part = a;
-    part.M = (a.M / 2 + 255) & ~255;
+    part.M = (int)done;
     rc = linear_rows_of(part, kp, stream);
     if (rc != 0) return rc;
     part = a;
-    const long long done = (a.M / 2 + 255) & ~255;
     part.M -= (int)done, part.q += done * a.ld_q, part.scale += done;
     part.out = (char*)a.out + done * a.ld_out * (a.dtype == F_FP32 ? 4 : 2);
     return linear_rows_of(part, kp, stream);
 }
 
 D4PG_API int d4pg_linear_int8(const LinearInt8Args* a, hipStream_t stream) {
-    if (a->M < 1 || a->N < 1 || a->N > 1 << 30 || a->K < 1 || a->K >= 131072) return -1;
+    if (a->M < 1 || a->N < 1 || a->N > 1 << 29 || a->K < 1 || a->K >= 131072) return -1;
     if (a->q == nullptr || a->w == nullptr || a->scale == nullptr || a->wscale == nullptr || a->out == nullptr) return -2;
     const long long kp = (a->K + 15) & ~15;
     if (((a->M > 1 ? a->ld_q : 16) & 15) || ((a->N > 1 ? a->ld_w : 16) & 15)) return -3;
@@ -916,7 +917,7 @@ __device__ __forceinline__ void lds_barrier() {          // LDS is settled for t
 }
 //
 // Measured (GPU time, us; the layers as launches of their own behind the /): 24-400-400-4 on one state 10.2 / 12.5, on 4096
-// states 12.7 / 30, on 8192 15.5 / 41; 111-1024-1024-8 on one state 18.6 / 13.8 (plus 22 of host time), on 4096 27.9 / 43, on
+// states 12.7 / 30, on 8192 15.5 / 41; 111-1024-1024-8 on one state 18.6 / 13.8 (whose six launches cost the host 20), on 4096 27.9 / 43, on
 // 8192 35.7 / 53.  At 4096 states of the latter 256 workgroups read 1.2 MB of weights each: 300 MB at the 18 TB/s that moves
 // alone reach would be 16 us.  At one state the chain of phases is what is left (clock stamps of a 400-wide network, cycles:
 // descriptors 2000, input 2400, layers 1200 + 4200 + 800, results and codes 1500 - 2500 each).

@@ -167,6 +167,21 @@ PyObject* dequantize(PyObject*, PyObject* const* o, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// One layer on rows that are not codes yet; an undefined tensor where an entry refused.
+Tensor coded_layer(const Tensor& x, const Weights& l, int act, int dtype, hipStream_t s) {
+    const int64_t M = x.size(0), K = x.size(1);
+    Tensor q = at::empty({M, padded(K)}, x.options().dtype(at::kChar)), scale = at::empty({M}, x.options().dtype(at::kFloat));
+    QuantRowsArgs r = {};
+    r.x = x.const_data_ptr(), r.q = static_cast<signed char*>(q.data_ptr()), r.scale = f32(scale);
+    r.M = M, r.K = K, r.ld_x = x.stride(0), r.ld_q = padded(K), r.dtype = float_code(x.scalar_type()), r.wdtype = F_NONE;
+    if (quant_rows(&r, s) != 0) return Tensor();
+    Tensor out = at::empty({M, l.N}, x.options().dtype(float_type(dtype)));
+    LinearInt8Args a = {};
+    a.q = r.q, a.scale = r.scale, a.w = l.w, a.wscale = l.scale, a.bias = l.bias, a.out = out.data_ptr();
+    a.ld_q = r.ld_q, a.ld_w = l.ld, a.ld_out = l.N, a.M = (int)M, a.N = (int)l.N, a.K = (int)K, a.act = act, a.dtype = dtype;
+    return linear_int8(&a, s) == 0 ? out : Tensor();
+}
+
 // mlp3(x, weight, weight_scale, bias, ... three times, activation code, type code)
 PyObject* mlp3(PyObject*, PyObject* const* o, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -177,20 +192,28 @@ PyObject* mlp3(PyObject*, PyObject* const* o, Py_ssize_t n) {
     const Tensor* x = dense(o[0], dev);
     if (!rows(x) || float_code(x->scalar_type()) == F_NONE || x->size(0) > INT_MAX) Py_RETURN_NONE;
     Mlp3Int8Args a = {};
+    Weights l[3];
     int64_t K = x->size(1);
     if (K > INT_MAX) Py_RETURN_NONE;
     a.width[0] = (int)K;
     for (int i = 0; i < 3; ++i) {
-        Weights l;
-        if (!layer(o + 1 + 3 * i, dev, K, l)) Py_RETURN_NONE;
-        a.w[i] = l.w, a.wscale[i] = l.scale, a.bias[i] = l.bias, a.ld_w[i] = l.ld;
-        K = l.N;
+        if (!layer(o + 1 + 3 * i, dev, K, l[i])) Py_RETURN_NONE;
+        a.w[i] = l[i].w, a.wscale[i] = l[i].scale, a.bias[i] = l[i].bias, a.ld_w[i] = l[i].ld;
+        K = l[i].N;
         a.width[i + 1] = (int)K;
     }
     Tensor out = at::empty({x->size(0), K}, x->options().dtype(float_type(dtype)));
     a.x = x->const_data_ptr(), a.ld_x = x->stride(0), a.out = out.data_ptr(), a.ld_out = K, a.M = (int)x->size(0);
     a.xdtype = float_code(x->scalar_type()), a.dtype = (int)dtype, a.act = (int)act;
-    if (mlp3_int8(&a, stream(dev)) != 0) Py_RETURN_NONE;
+    const hipStream_t s = stream(dev);
+    const int rc = mlp3_int8(&a, s);
+    if (rc == 1) {               // wider than its LDS: a launch a step
+        out = *x;
+        for (int i = 0; i < 3 && out.defined(); ++i) out = coded_layer(out, l[i], i < 2 ? ACT_RELU : (int)act, i < 2 ? F_FP32 : (int)dtype, s);
+        if (!out.defined()) Py_RETURN_NONE;
+    } else if (rc != 0) {
+        Py_RETURN_NONE;
+    }
     return THPVariable_Wrap(std::move(out));
     END_HANDLE_TH_ERRORS
 }

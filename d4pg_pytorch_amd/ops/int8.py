@@ -30,6 +30,7 @@ _ACTS = {"none": H.ACT_NONE, "relu": H.ACT_RELU, "tanh": H.ACT_TANH}
 #: products of two codes are at most 128^2 in magnitude: sums of this many fit 32 bits
 MAX_K = 131071
 _F32, _I8 = torch.float32, torch.int8
+_MOST = 2 ** 31 - 1
 
 
 #: the plain case of every operator in C++ (``csrc/int8_bind.cpp``; loaded with the first GPU tensor).  What it returns
@@ -79,6 +80,8 @@ def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
     K = x.shape[1]
     if K < 1:
         raise ValueError(f"{what} needs at least one column, not shape {tuple(x.shape)}")
+    if x.shape[0] > _MOST or K > _MOST:
+        raise ValueError(f"{what}: {x.shape[0]} rows of {K} elements are more than 2^31 - 1 of either")
     return x if K == 1 or x.stride(1) == 1 else x.contiguous()
 
 
@@ -236,8 +239,8 @@ def _layer(device: torch.device, K: int, weight: torch.Tensor, weight_scale: tor
         raise ValueError(f"weight has shape {tuple(weight.shape)}, expected (out, {K})")
     if K > MAX_K:
         raise ValueError(f"{K} columns: sums of more than {MAX_K} products can leave 32 bits")
-    if weight.shape[0] > 1 << 30:
-        raise ValueError(f"{weight.shape[0]} outputs: at most 2^30 are supported")
+    if weight.shape[0] > 1 << 29:
+        raise ValueError(f"{weight.shape[0]} outputs: at most 2^29 are supported")
     _on(device, "weight", weight)
     outs = weight.shape[:1]
     return _vector(device, "weight_scale", weight_scale, outs), None if bias is None else _vector(device, "bias", bias, outs)

@@ -354,6 +354,12 @@ def test_refusals(device):
     long_q = torch.zeros(1, 131072, dtype=torch.int8, **d)
     with pytest.raises(ValueError, match="32 bits"):
         ops.linear_int8(long_q, s[:1], long_q, s[:1])
+    one = torch.zeros(1, **d)
+    for shape in ((1 << 31, 1), (1, 1 << 31)):
+        with pytest.raises(ValueError, match="2.31"):
+            ops.quantize_rows(one.expand(*shape))
+    with pytest.raises(ValueError, match="2.29"):
+        ops.linear_int8(q[:, :1], s, one.to(torch.int8).expand((1 << 29) + 1, 1), one.expand((1 << 29) + 1))
     with pytest.raises(ValueError):
         ops.mlp3_int8(x, ((w, ws, None),) * 2)
     with pytest.raises(ValueError):
@@ -582,7 +588,7 @@ def test_the_library_refuses_what_its_kernels_cannot_read():
             setattr(a, k, v)
         return lib.d4pg_linear_int8(C.byref(a), None)
 
-    for kw in (dict(M=0), dict(N=0), dict(N=(1 << 30) + 1), dict(K=0), dict(K=131072), dict(q=None), dict(w=None), dict(scale=None), dict(wscale=None),
+    for kw in (dict(M=0), dict(N=0), dict(N=(1 << 29) + 1), dict(K=0), dict(K=131072), dict(q=None), dict(w=None), dict(scale=None), dict(wscale=None),
                dict(out=None), dict(ld_q=40), dict(ld_w=24), dict(ld_q=16), dict(ld_w=16), dict(ld_out=3), dict(q=4104), dict(w=8193),
                dict(dtype=3), dict(dtype=-1), dict(act=3), dict(act=-1)):
         assert product(**kw) < 0, kw
