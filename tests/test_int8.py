@@ -472,6 +472,65 @@ def test_a_residual_block_of_them(device):
     assert (y.double() - y64).norm() <= 0.05 * y64.norm()
 
 
+class _Declines:
+    """A binding that leaves everything to the Python way."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+@pytest.mark.gpu
+def test_the_binding_and_the_python_way_agree(monkeypatch):
+    from d4pg_pytorch_amd.ops import int8
+    x, r = _randn(70, 333, seed=1).cuda(), _randn(70, 333, seed=2).cuda()
+    g = _randn(333, seed=3).cuda()
+    narrow = _layers(((130, 333), (130, 130), (9, 130)), "cuda")
+    wide = _layers(((1300, 333), (40, 1300), (9, 40)), "cuda", bias=False)
+
+    def everything():
+        q, s, h = ops.add_rms_norm_int8(x, g, r, 1e-5)
+        p, t, same = ops.add_rms_norm_int8(x.half(), eps=0)
+        c, u = ops.quantize_rows(x.bfloat16())
+        w, ws, b = narrow[0]
+        return (q, s, h, p, t, same, c, u, ops.dequantize_rows(c, u, torch.float16), ops.linear_int8(q, s, w, ws, b, "tanh", torch.bfloat16),
+                ops.mlp3_int8(x, narrow, "tanh"), ops.mlp3_int8(x, wide, "relu", torch.float16), ops.mlp3_int8(x, narrow, "softmax"))
+
+    fast = everything()
+    with torch.inference_mode():
+        again = everything()
+    monkeypatch.setattr(int8, "_plain", _Declines())
+    slow = everything()
+    for a, b, c in zip(fast, slow, again):
+        assert a.dtype == b.dtype and a.shape == b.shape and a.stride() == b.stride()
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@pytest.mark.gpu
+def test_calls_from_several_threads_on_streams_of_their_own():
+    import threading
+    layers = _layers(((256, 100), (256, 256), (5, 256)), "cuda")
+    xs = [_randn(300, 100, seed=i).cuda() for i in range(4)]
+    want = [ops.mlp3_int8(x, layers, "tanh") for x in xs]
+    lin = [ops.linear_int8(*ops.quantize_rows(x), *layers[0]) for x in xs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                y = ops.mlp3_int8(xs[i], layers, "tanh")
+                z = ops.linear_int8(*ops.quantize_rows(xs[i]), *layers[0])
+                if not (torch.equal(y, want[i]) and torch.equal(z, lin[i])):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not bad
+
+
 @pytest.mark.gpu
 def test_more_rows_than_one_launch_holds():
     """64 threads a row: 2^26 rows are 2^32 threads, which is one too many for a launch; offsets pass 32 bits too."""
