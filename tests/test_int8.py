@@ -224,6 +224,18 @@ def _check_linear(y, q, scale, w, ws, b, act, dtype):
     assert y.dtype == dtype and y.shape == want.shape and not bad.any(), f"{int(bad.sum())} of {bad.numel()} values"
 
 
+@pytest.mark.gpu
+def test_tanh_over_its_whole_range():
+    """One column: the sum times its scale is the argument itself.  5 steps of fp32 are allowed (10 u)."""
+    v = torch.cat([torch.linspace(-12, 12, 200001), torch.logspace(-30, 4, 50001), -torch.logspace(-30, 4, 50001), torch.linspace(-0.6, 0.6, 100001),
+                   torch.tensor([0.0, 0.5, -0.5, 1e-40, -1e-40, 3e38, math.inf, -math.inf, math.nan])]).cuda()
+    one = torch.ones(v.numel(), 1, dtype=torch.int8, device="cuda")
+    y = ops.linear_int8(one, v, one[:1], torch.ones(1, device="cuda"), None, "tanh")[:, 0]
+    want = torch.tanh(v.double())
+    assert torch.isnan(y[-1]) and torch.all((y[:-1].double() - want[:-1]).abs() <= 10 * U * want[:-1].abs() + 2.0 ** -149)
+    assert torch.all(y[:-1].abs() <= 1)
+
+
 SHAPES = [(1, 1, 1), (1, 3, 15), (2, 4, 16), (1, 400, 400), (3, 5, 17), (16, 16, 64), (17, 33, 65), (1, 50, 1000), (5, 17, 127),
           (31, 31, 129), (64, 51, 400), (65, 64, 256), (128, 128, 128), (129, 130, 131), (256, 400, 400), (300, 7, 2001),
           (7, 300, 2001), (257, 513, 640), (500, 260, 1111), (2, 4096, 1024), (1030, 1025, 385), (40, 2050, 96)]
