@@ -831,9 +831,10 @@ static int launch_linear_tiles(const LinearInt8Args& a, hipStream_t stream) {
     return (int)hipGetLastError();
 }
 
-// Which kernel.  Tiles are taken from the largest size that still gives most of the 256 CUs one; below 128 tiles of 64 x 64 and
-// up to 32 rows the rows kernel, whose workgroups split K instead.  Few tiles with a long K get more waves and four steps of
-// moves in flight, which hides the way from memory; with a short K or many tiles two steps and more workgroups a CU do better.
+// Which kernel.  Tiles are taken from the largest size that still gives most of the 256 CUs one and is not more than twice as
+// tall as there are rows (17 - 32 rows: 64 x 64 only with a long K); below 128 tiles of 64 x 64 and up to 16 rows the rows
+// kernel, whose workgroups split K instead.  Few tiles with a long K get more waves and four steps of moves in flight, which
+// hides the way from memory; with a short K or many tiles two steps and more workgroups a CU do better.
 // Measured on an MI355X, us (graph of 20 calls on three sets of operands in turn, median; tiles of that size in brackets):
 //     tile, waves, steps in LDS   for                            and by the neighbouring choice
 //     256 x 256, 16, 2            2048 x 8192 x 8192  (256)  124   155 with 128 x 128;  2048 x 4096 x 4096 (128)  52 / 43
@@ -849,6 +850,10 @@ static int launch_linear_tiles(const LinearInt8Args& a, hipStream_t stream) {
 //     64 x 64,  4, 2              2048 x 1024 x 1024  (512)   9.4  10.5 with K halved; 11.7 with 128 x 128
 //                                 1280 x 1024 x 512   (320)   5.7  6.1 with K halved;  with K = 1024  8.2 / 7.9
 //                                 512 x 1024 x 512    (128)   4.9  5.7 with rows;  with K = 1024 (K halved)  5.8 / 5.6
+//     few rows, many columns      128 x 49152 x 1024  128 x 128  16.2, 256 x 256  23.0;  128 x 65536 x 4096  81 and 85
+//                                 64 x 65536 x 4096   64 x 64  62, 128 x 128  71, 256 x 256  82;  65 x 18432 x 4096  24 and 19.5, -
+//                                 32 x 18432 x 4096   64 x 64  17.9, 128 x 128  19.1, rows  24.9;  32 x 16384 x 1024  7.3, -, rows  6.8
+//                                 1 x 65536 x 4096    rows  59, 64 x 64  57, 128 x 128  66, 256 x 256  72;  1 x 18432 x 4096  18.2, 16.7, 18.0, -
 // Between the row kernels the number of 16 x 16 tiles decides: as many columns and rows a workgroup as leave 200 - 400
 // workgroups (one set of operands, 256 x 400 x 400: 3.7 with 2 x 1 tiles, 4.0 with 1 x 1, 4.2 with 2 x 2; 512 x 1024 x 1024: 6.3 with 4 x 2, 6.9
 // with 2 x 2, 8.6 with 2 x 1; 1 x 16384 x 4096: 12.8 with 1 x 4, 14.6 with 1 x 1), and K is dealt to 16 waves where it is long
@@ -857,10 +862,10 @@ static int launch_linear(const LinearInt8Args& a, long long kp, hipStream_t stre
     auto tiles = [&](int side) { return (long long)((a.M + side - 1) / side) * ((a.N + side - 1) / side); };
     // the tile kernel's offsets inside 256 rows are 32-bit
     if (256 * (a.M > 1 ? a.ld_q : kp) + kp < 0x7fffffffll && 256 * (a.N > 1 ? a.ld_w : kp) + kp < 0x7fffffffll) {
-        if (tiles(256) >= 192) return launch_linear_tiles<2, 2, 4, 4, 1, 2>(a, stream);
-        if (tiles(128) > 256) return launch_linear_tiles<2, 1, 2, 4, 1, 2>(a, stream);
-        if (tiles(128) >= 144 && a.K >= 2048) return launch_linear_tiles<1, 1, 4, 4, 1, 4>(a, stream);
-        if (a.M > 32 && tiles(64) >= 128) {
+        if (a.M > 128 && tiles(256) >= 192) return launch_linear_tiles<2, 2, 4, 4, 1, 2>(a, stream);
+        if (a.M > 64 && tiles(128) > 256) return launch_linear_tiles<2, 1, 2, 4, 1, 2>(a, stream);
+        if (a.M > 64 && tiles(128) >= 144 && a.K >= 2048) return launch_linear_tiles<1, 1, 4, 4, 1, 4>(a, stream);
+        if ((a.M > 32 && tiles(64) >= 128) || (a.M > 16 && tiles(64) >= 256 && a.K >= 2048)) {
             if (a.K >= 4096 || (a.K >= 1024 && tiles(64) <= 384)) return launch_linear_tiles<1, 1, 2, 2, 2, 4>(a, stream);
             return launch_linear_tiles<1, 1, 2, 2, 1, 2>(a, stream);
         }

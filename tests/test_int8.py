@@ -250,6 +250,17 @@ def test_linear_int8_by_every_kernel(M, N, K):
     _linear_case(M, N, K, "cuda")
 
 
+#: large tiles with a long and a short K; few rows and many columns, at both sides of 16, 32, 64 and 128 rows
+WIDE_SHAPES = [(1800, 1700, 2050), (2200, 2300, 150), (1, 18500, 2049), (16, 18500, 2100), (17, 18500, 2049), (32, 17000, 2100), (33, 18500, 2049),
+               (64, 33000, 40), (65, 33000, 40), (65, 18500, 2049), (128, 49300, 40), (129, 49300, 40), (3, 66000, 40)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", WIDE_SHAPES)
+def test_linear_int8_with_many_columns(M, N, K):
+    _linear_case(M, N, K, "cuda")
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("M,N,K", SHAPES)
 def test_linear_int8(M, N, K, device):
