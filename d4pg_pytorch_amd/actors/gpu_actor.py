@@ -167,8 +167,15 @@ class GpuActor:
 
     # ------------------------------------------------------------------ weights
     def _quantize(self) -> None:
-        """Codes of the parameters in ``flat``, per output channel.  Enqueue only."""
-        self.codes = tuple((*quantize_rows(w), b) for w, b in zip(self.view.weights, self.view.biases))
+        """Codes of the parameters in ``flat``, per output channel, always in the same memory: a captured ``act_device``
+        follows the weights, as the fp32 kernels do.  Enqueue only."""
+        new = tuple((*quantize_rows(w), b) for w, b in zip(self.view.weights, self.view.biases))
+        if self.codes is None:
+            self.codes = new
+            return
+        for (q, scale, _), (q_new, scale_new, _) in zip(self.codes, new):
+            q.copy_(q_new)
+            scale.copy_(scale_new)
 
     def load_flat(self, flat) -> None:
         self._flat_host.copy_(torch.as_tensor(np.asarray(flat, dtype=np.float32)))

@@ -628,6 +628,39 @@ def test_a_gpu_agent_acts_on_8_bit_codes(S, A, Hd, E):
         GpuActor(S, A, Hd, precision="int4")
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("Hd", [64, 1100])
+def test_a_captured_policy_follows_new_parameters(Hd):
+    from d4pg_pytorch_amd.actors.gpu_actor import GpuActor
+    from d4pg_pytorch_amd.models.nets import ActorPolicy, init_net_
+    S, A, E = 11, 3, 5
+    pol = ActorPolicy(S, A, Hd)
+    init_net_(pol.view, 0.05, _gen(3))
+    ga = GpuActor(S, A, Hd, max_batch=E, precision="int8")
+    ga.load_flat(pol.flat.numpy())
+    places = [t.data_ptr() for layer in ga.codes for t in layer]
+    obs, out = _randn(E, S, seed=4).cuda(), torch.zeros(E, A, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ga.act_device(obs, out)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ga.act_device(obs, out)
+    seen = []
+    for seed in (5, 6, 7):
+        init_net_(pol.view, 0.05, _gen(seed))
+        ga.load_flat(pol.flat.numpy())
+        assert places == [t.data_ptr() for layer in ga.codes for t in layer]
+        graph.replay()
+        got = out.clone()
+        fresh = [(*ops.quantize_rows(w.cuda()), b.cuda()) for w, b in zip(pol.view.weights, pol.view.biases)]
+        assert torch.equal(got, ops.mlp3_int8(obs, fresh, "tanh"))
+        seen.append(got)
+    assert not torch.equal(seen[0], seen[1]) and not torch.equal(seen[1], seen[2])
+
+
 def test_the_agents_precision_is_a_config_key():
     from d4pg_pytorch_amd.config import ConfigError, default_config
     assert default_config(env="Pendulum-v0")["policy_precision"] == "fp32"
