@@ -52,11 +52,13 @@ __device__ __forceinline__ unsigned row16_umax(unsigned v) {       // over 16 ne
     v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false));
     return v;
 }
+// The same bits in all 16 lanes: every step adds two values that both partners hold (neighbours, pairs, quads mirrored in 8
+// lanes, eights mirrored in 16).  Rotations by 4 and 8 would pair the quads differently in the two halves of the row.
 __device__ __forceinline__ float row16_sum(float v) {
     v += dpp_mov<0xb1>(v);
     v += dpp_mov<0x4e>(v);
-    v += dpp_mov<0x124>(v);
-    v += dpp_mov<0x128>(v);
+    v += dpp_mov<0x141>(v);
+    v += dpp_mov<0x140>(v);
     return v;
 }
 __device__ __forceinline__ unsigned wave_umax(unsigned v) {

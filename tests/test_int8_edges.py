@@ -1,0 +1,32 @@
+"""8-bit serving operators (``ops/int8.py``, ``csrc/int8.hip``) at borders of their arithmetic, their dispatch and their
+calls.  Bounds as in ``test_int8.py``, whose helpers these tests use."""
+import math
+
+import pytest
+import torch
+
+from d4pg_pytorch_amd import ops
+from test_int8 import DEVICES, NORM, _check_codes, _norm64, _randn
+
+
+# --------------------------------------------------------------------------------------------- the norm's two branches
+@pytest.mark.parametrize("device", DEVICES)
+def test_norm_whose_sum_of_squares_is_at_the_end_of_fp32(device):
+    """By one order of additions the sum of these squares is the largest fp32 number, by another it is infinite: the
+    threads of the row have to agree on one."""
+    x = torch.zeros(1, 128)
+    x[0, 0], x[0, 32], x[0, 64], x[0, 96] = (float.fromhex(v) for v in ("0x1.000004p+63", "0x1.fffffep+62", "0x1p+63", "0x1.fffff6p+62"))
+    q, scale, _ = ops.add_rms_norm_int8(x.to(device))
+    assert q[0, ::32].tolist() == [127] * 4
+    _check_codes(q, scale, _norm64(x, None, None, 1e-6)[1], NORM)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("K", [9, 77, 128, 250, 400, 3001])
+def test_norm_around_the_smallest_plain_mean_square(K, device):
+    """Rows whose mean square passes 2^-80 in steps of the last place."""
+    base = _randn(60, K, seed=K).double()
+    base = base * (2.0 ** -40 / base.square().mean(1, keepdim=True).sqrt())
+    x = torch.cat([base * (1 + j * 2.0 ** -25) for j in range(-12, 13)]).float()
+    q, scale, _ = ops.add_rms_norm_int8(x.to(device), eps=0.0)
+    _check_codes(q, scale, _norm64(x, None, None, 0.0)[1], NORM)
