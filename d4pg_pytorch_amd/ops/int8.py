@@ -72,7 +72,9 @@ def _on(device: torch.device, what: str, t: torch.Tensor) -> None:
 
 
 def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
-    """``x[..., K]`` as ``[M, K]`` with neighbouring elements side by side."""
+    """``x[..., K]`` as ``[M, K]`` with neighbouring elements side by side, in memory as they read (a view whose sign is
+    pending, such as ``z.conj().imag``, is copied)."""
+    x = x.resolve_neg()
     if x.ndim != 2:
         if x.ndim < 1 or x.shape[-1] < 1:
             raise ValueError(f"{what} needs at least one column, not shape {tuple(x.shape)}")
@@ -122,7 +124,7 @@ def _vector(device: torch.device, what: str, s: torch.Tensor, shape) -> torch.Te
         if not s.is_floating_point():
             raise TypeError(f"{what} must be a floating tensor, not {s.dtype}")
         s = s.float()
-    return s if s.is_contiguous() else s.contiguous()
+    return s.resolve_neg().contiguous()
 
 
 def _codes_given(q: torch.Tensor, what: str) -> None:
@@ -214,7 +216,7 @@ def add_rms_norm_int8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, re
             raise ValueError(f"weight has shape {tuple(weight.shape)}, expected ({K},)")
         wt = _float_code(weight, "weight")
         _on(device, "weight", weight)
-        weight = weight.contiguous()
+        weight = weight.resolve_neg().contiguous()
     if not x.is_cuda:
         with torch.no_grad():
             q, scale, h = ref.add_rms_norm_int8(x2, weight, r2, eps)

@@ -30,3 +30,36 @@ def test_norm_around_the_smallest_plain_mean_square(K, device):
     x = torch.cat([base * (1 + j * 2.0 ** -25) for j in range(-12, 13)]).float()
     q, scale, _ = ops.add_rms_norm_int8(x.to(device), eps=0.0)
     _check_codes(q, scale, _norm64(x, None, None, 0.0)[1], NORM)
+
+
+# ------------------------------------------------------------------------------------------- views whose sign is pending
+@pytest.mark.parametrize("device", DEVICES)
+def test_views_whose_sign_is_pending(device):
+    """``torch._neg_view(t)`` holds ``t`` in memory and reads as ``-t``; so does the imaginary part of a conjugate."""
+    def pending(t):
+        view = torch._neg_view(t)
+        assert view.is_neg()
+        return view
+
+    x, r, g = (_randn(*shape, seed=i).to(device) for i, shape in enumerate(((5, 40), (5, 40), (40,))))
+    z = torch.complex(x[:, :1], r[:, :1]).conj().imag
+    assert z.is_neg() and z.shape == (5, 1)
+
+    def same(a, b):
+        assert all(torch.equal(s, t) for s, t in zip(a, b))
+
+    same(ops.quantize_rows(pending(x)), ops.quantize_rows(-x))
+    same(ops.quantize_rows(z), ops.quantize_rows(-r[:, :1]))
+    same(ops.add_rms_norm_int8(pending(x), pending(g), pending(r)), ops.add_rms_norm_int8(-x, -g, -r))
+    same(ops.add_rms_norm_int8(x, pending(g)), ops.add_rms_norm_int8(x, -g))
+    q, s = ops.quantize_rows(x)
+    w, ws = ops.quantize_rows(_randn(7, 40, seed=5).to(device))
+    b = _randn(7, seed=6).to(device)
+    same([ops.dequantize_rows(pending(q), pending(s))], [ops.dequantize_rows(-q, -s)])
+    for args in ((pending(q), s, w, ws, b), (q, pending(s), w, ws, b), (q, s, pending(w), ws, b), (q, s, w, pending(ws), b),
+                 (q, s, w, ws, pending(b))):
+        same([ops.linear_int8(*args)], [ops.linear_int8(*(a.resolve_neg() for a in args))])
+    layers = [(*ops.quantize_rows(_randn(n, k, seed=n).to(device)), _randn(n, seed=k).to(device)) for n, k in ((16, 40), (16, 16), (3, 16))]
+    same([ops.mlp3_int8(pending(x), layers)], [ops.mlp3_int8(-x, layers)])
+    turned = [(w, pending(-ws), pending(-b)) for w, ws, b in layers]
+    same([ops.mlp3_int8(x, turned)], [ops.mlp3_int8(x, layers)])
