@@ -139,7 +139,7 @@ struct NormFactor {
 };
 __device__ __forceinline__ bool norm_is_plain(float ss, float K, float eps) {
     const float ms = ss / K + eps;
-    return ms >= 0x1p-80f && ss < __builtin_inff();
+    return ms >= 0x1p-80f && ms < __builtin_inff() && ss < __builtin_inff();
 }
 __device__ __forceinline__ float norm_lift(unsigned top_bits, float eps) {
     int e = (int)(top_bits >> 23) - 126;

@@ -18,6 +18,7 @@ scale 0 and codes 0.
 """
 from __future__ import annotations
 
+import ctypes as C
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -193,15 +194,15 @@ def add_rms_norm_int8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, re
 
     ``x[..., K]`` and ``residual`` (same shape and type, or ``None``: then ``h`` is ``x`` itself) are fp32, bf16 or fp16;
     ``weight[K]`` any of them, or ``None`` for ones.  The norm is of the fp32 sum; ``h`` is that sum rounded to the type
-    of ``x``.  ``mean`` and everything up to the codes is fp32."""
+    of ``x``.  ``mean`` and everything up to the codes is fp32, ``eps`` too (what fp32 does not hold is refused)."""
     if x.is_cuda:
         out = _binding().quantize(x, weight, residual, eps)
         if out is not None:
             return out
     dt = _float_code(x, "x")
-    eps = float(eps)
-    if not 0.0 <= eps < float("inf"):
-        raise ValueError(f"eps must be a finite number >= 0, not {eps}")
+    given, eps = eps, C.c_float(eps).value
+    if not (given >= 0.0 and eps < float("inf")):
+        raise ValueError(f"eps must be a number >= 0 that fp32 holds, not {given}")
     device = x.device
     x2 = _rows(x, "x")
     M, K = x2.shape

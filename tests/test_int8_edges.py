@@ -63,3 +63,26 @@ def test_views_whose_sign_is_pending(device):
     same([ops.mlp3_int8(pending(x), layers)], [ops.mlp3_int8(-x, layers)])
     turned = [(w, pending(-ws), pending(-b)) for w, ws, b in layers]
     same([ops.mlp3_int8(x, turned)], [ops.mlp3_int8(x, layers)])
+
+
+# ---------------------------------------------------------------------------------------------- the ends of eps's range
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("K", [1, 40, 700, 40000])
+def test_norm_with_an_eps_at_the_ends_of_fp32(K, device):
+    """``mean + eps`` may pass the largest fp32 number though both are finite; ``eps`` below 2^-150 is nothing."""
+    top = torch.finfo(torch.float32).max
+    x = torch.cat([_randn(2, K, seed=K), 1e19 / math.sqrt(K) * _randn(2, K, seed=1), 1e-30 * _randn(2, K, seed=2)])
+    for eps in (top, 3.3e38, 2.0 ** -149, 2.0 ** -126):
+        q, scale, _ = ops.add_rms_norm_int8(x.to(device), eps=eps)
+        rows = [0, 1, 4, 5] if eps < 1 else [0, 1, 2, 3]
+        _check_codes(q[rows], scale[rows], _norm64(x[rows], None, None, eps)[1], NORM)
+    q, scale, _ = ops.add_rms_norm_int8(x.to(device), eps=1e-50)
+    _check_codes(q, scale, _norm64(x, None, None, 0.0)[1], NORM)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusal_of_an_eps_that_fp32_does_not_hold(device):
+    x = _randn(2, 8).to(device)
+    for eps in (3.5e38, 1e300, 10.0 ** 60, -1e-30, -1e-60, -math.inf):
+        with pytest.raises(ValueError, match="eps"):
+            ops.add_rms_norm_int8(x, eps=eps)
