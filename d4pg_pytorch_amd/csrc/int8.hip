@@ -100,25 +100,29 @@ __device__ __forceinline__ unsigned abs_bits(float v) { return __builtin_bit_cas
 // What turns a row's values into codes.  |y| as an unsigned integer orders like the value, with infinity and NaN above
 // every finite number, so one integer maximum finds the largest magnitude and whether the row is finite.
 struct RowCode {
-    float pre, inv, scale;
+    float pre, inv, rest, scale;       // 127 / (top * pre) = inv + rest
     unsigned keep;         // all ones, or 0 for a row that is not finite
 };
 __device__ __forceinline__ RowCode row_code(unsigned top_bits) {
     const float top = __builtin_bit_cast(float, top_bits);
     RowCode c;
-    const bool finite = top_bits < 0x7f800000u;
-    // 127 / top overflows for the smallest rows: those are lifted by 2^64 first (exact)
-    c.pre = top < 0x1p-62f ? 0x1p64f : 1.f;
-    c.inv = top > 0.f && finite ? 127.f / (top * c.pre) : 0.f;
+    const bool finite = top_bits < 0x7f800000u, some = top > 0.f && finite;
+    // the smallest and the largest rows are moved by 2^64 first (exact), where 127 / top or its rest would leave fp32
+    c.pre = top < 0x1p-62f ? 0x1p64f : top > 0x1p62f ? 0x1p-64f : 1.f;
+    const float a = top * c.pre;
+    c.inv = some ? 127.f / a : 0.f;
+    c.rest = some ? __builtin_fmaf(-c.inv, a, 127.f) * (c.inv * (1.f / 127.f)) : 0.f;
     c.scale = finite ? top / 127.f : __builtin_nanf("");
     c.keep = finite ? ~0u : 0u;
     return c;
 }
-// rint(y * 127 / a) as a byte: adding 1.5 * 2^23 leaves the rounded integer, halves to even, in the low bits.  The product is
-// rounded on its own: where y / a is exactly halfway between two codes that restores the half which 127 / a had lost.
+// y * 127 / a, rounded to fp32, then to the nearest whole number, halves to even, as a byte.  127 / a in one fp32 number would
+// move the halves (a / 2 is 63.5 codes whatever a is): with its rest the product's error is 2^-47 before the fma rounds it,
+// so that a quotient which is exactly halfway stays there.  Adding 1.5 * 2^23 leaves the whole number in the low bits.
+// One instruction a value more than without the rest: 65536 x 100 fp32 8.7 -> 8.9 us, longer rows and the policy within 1 %.
 __device__ __forceinline__ unsigned code_bits(float y, const RowCode& c) {
 #pragma clang fp contract(off)
-    const float v = y * c.pre * c.inv;
+    const float x = y * c.pre, v = __builtin_fmaf(x, c.inv, x * c.rest);
     return __builtin_bit_cast(unsigned, v + 12582912.f);
 }
 __device__ __forceinline__ unsigned pack4(unsigned a, unsigned b, unsigned c, unsigned d) {

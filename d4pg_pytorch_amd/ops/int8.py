@@ -146,7 +146,8 @@ def _shaped(t: torch.Tensor, x: torch.Tensor, *last: int) -> torch.Tensor:
 
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """``x[..., K]`` (fp32 / bf16 / fp16) -> ``(codes[..., K] int8, scale[...] fp32)``:
-    ``scale = max |row| / 127``, ``code = round(x * 127 / max |row|)``, halves to even."""
+    ``scale = max |row| / 127``, ``code = round(x * 127 / max |row|)``, the quotient rounded to fp32 and then to the nearest
+    whole number, halves to even."""
     if x.is_cuda:
         out = _binding().quantize(x)
         if out is not None:

@@ -278,15 +278,14 @@ def mlp3(x, w1, b1, w2, b2, w3, b3, final: str = "none"):
 
 
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
-    """``scale = max |row| / 127``, ``code = round(x * 127 / max |row|)``.  A row of zeros: scale 0, codes 0; a row
+    """``scale = max |row| / 127``, ``code = round(x * 127 / max |row|)``, halves to even.  A row of zeros: scale 0, codes 0; a row
     with a NaN or an infinity: scale NaN, codes 0."""
     x = x.float()
     top = x.abs().amax(dim=1, keepdim=True)
     finite = torch.isfinite(top)
-    # the smallest rows are lifted by 2^64 first: 127 / top would overflow
-    pre = torch.where(top < 2.0 ** -62, torch.full_like(top, 2.0 ** 64), torch.ones_like(top))
-    inv = torch.where(finite & (top > 0), 127.0 / (top * pre), torch.zeros_like(top))
-    codes = torch.where(finite, torch.round(x * pre * inv), torch.zeros_like(x))
+    # the quotient from 64 bits, rounded to fp32, then to a whole number (halves to even)
+    v = (x.double() * 127.0 / top.double()).float()
+    codes = torch.where(finite & (top > 0), torch.round(v), torch.zeros_like(x))
     scale = torch.where(finite, top / 127.0, torch.full_like(top, math.nan))
     return codes.to(torch.int8), scale[:, 0]
 

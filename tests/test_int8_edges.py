@@ -86,3 +86,57 @@ def test_refusal_of_an_eps_that_fp32_does_not_hold(device):
     for eps in (3.5e38, 1e300, 10.0 ** 60, -1e-30, -1e-60, -math.inf):
         with pytest.raises(ValueError, match="eps"):
             ops.add_rms_norm_int8(x, eps=eps)
+
+
+# ------------------------------------------------------------------------------------------------- codes, to the last one
+def _codes_of(x):
+    """Codes of rows of whole numbers ``x`` [M, K] (int64, below 2^24), in whole numbers throughout."""
+    top = x.abs().amax(1, keepdim=True)
+    doubled = 254 * x.abs()                       # of 2 top: code = floor((254 |x| + top) / (2 top)), a half to the even one
+    k = (doubled + top) // (2 * top)
+    half = (doubled + top) % (2 * top) == 0
+    k = k - (half & (k % 2 == 1)).long()
+    return x.sign() * k
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("shift", [-149, -126, -90, -63, -62, -40, 0, 40, 62, 63, 100, 103])
+def test_halves_go_to_the_even_code(shift, device):
+    """Rows 2 x 127 m with every half there is, (2 k + 1) m, and its neighbours; and a / 2, which is 63.5 codes of any a."""
+    m = torch.tensor([1, 2, 3, 5, 7, 9, 11, 100, 333, 1023, 1025, 4099, 20011, 33023, 66047])[:, None]
+    halves = (2 * torch.arange(0, 127)[None] + 1) * m
+    x = torch.cat([254 * m, halves, -halves, halves + 1, 1 - halves, halves - 1], 1)
+    assert int(x.abs().max()) < 1 << 24
+    values = (x.double() * 2.0 ** shift).float()
+    assert torch.equal(values.double(), x.double() * 2.0 ** shift)
+    q, scale = ops.quantize_rows(values.to(device))
+    assert torch.equal(q.cpu().long(), _codes_of(x))
+    assert torch.equal(scale.cpu(), values[:, 0] / 127)
+    a = torch.randint(1, 1 << 23, (500, 1), generator=torch.Generator().manual_seed(3)) * 2
+    x = torch.cat([a, a // 2, -(a // 2)], 1)
+    q, _ = ops.quantize_rows((x.double() * 2.0 ** shift).float().to(device))
+    assert torch.equal(q.cpu(), torch.tensor([127, 64, -64], dtype=torch.int8).expand(500, 3))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype,most", [(torch.bfloat16, 256), (torch.float16, 2048), (torch.float32, 1 << 24)])
+@pytest.mark.parametrize("K", [33, 500, 5000])
+def test_codes_of_whole_numbers(K, dtype, most, device):
+    """Every code of rows that the type holds exactly.  An fp32 quotient within 2^-18 of a half, but not on it, may be
+    rounded onto it: such places (at most 254 x 2^-18 x 2 of the values) are left out, for 16-bit types there are none."""
+    x = torch.randint(-most, most + 1, (64, K), generator=torch.Generator().manual_seed(K))
+    q, _ = ops.quantize_rows(x.to(dtype).to(device))
+    want = _codes_of(x)
+    v = x.double() * 127 / x.abs().amax(1, keepdim=True).double()
+    off = (v - v.floor() - 0.5).abs()
+    skip = (off > 0) & (off < 2.0 ** -18)
+    assert dtype == torch.float32 or not skip.any()
+    assert torch.equal(torch.where(skip, want, q.cpu().long()), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_both_devices_make_the_same_codes(dtype):
+    x = (_randn(300, 700, seed=1) * torch.exp(20 * _randn(300, 1, seed=2)).clamp(1e-3, 1e3)).to(dtype)
+    for a, b in zip(ops.quantize_rows(x), ops.quantize_rows(x.cuda())):
+        assert torch.equal(a, b.cpu())
