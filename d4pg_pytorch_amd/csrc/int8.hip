@@ -537,9 +537,10 @@ __device__ __forceinline__ Columns4 columns4(const float* wscale, const float* b
 __device__ __forceinline__ f32x4 scaled4(const i32x4 sum, float sm) {
     return f32x4{(float)sum[0] * sm, (float)sum[1] * sm, (float)sum[2] * sm, (float)sum[3] * sm};
 }
-// tanh x = sign x (1 - 2 / (e^2|x| + 1)), below 1/2, where that cancels, the Taylor series x - x^3 / 3 + 2 x^5 / 15 - ... to
-// x^15.  Measured over 4.5 million arguments against 64 bits: 0.77 units of the last place below 1/2, 2.6 above.
-// 777 x 1333 x 2001 takes 11.0 us with it and 11.6 with tanhf (fp16 results; 10.1 with ReLU), 256 x 400 x 400 3.90 and 4.03.
+// tanh for 16-bit results: sign x (1 - 2 / (e^2|x| + 1)), below 1/2, where that cancels, the Taylor series
+// x - x^3 / 3 + 2 x^5 / 15 - ... to x^15.  Over every fp32 argument of [0.001, 20) against 64 bits: at most 0.79 units of the
+// last place of fp32 below 1/2 and 2.6 above, which 16 bits do not hold.  fp32 results take tanhf (1.4 units over the same
+// arguments), which costs more: fp32 results of 777 x 1333 x 2001 12.8 us, 12.3 with this form; of 256 x 400 x 400 3.8 and 3.6.
 __device__ __forceinline__ float tanh_of(float x) {
     const float a = __builtin_fabsf(x), s = x * x;
     const float e = __builtin_amdgcn_exp2f(a * 2.8853900817779268f);       // 2 / ln 2
@@ -553,7 +554,7 @@ __device__ __forceinline__ float tanh_of(float x) {
     p = __builtin_fmaf(p, s, -1.f / 3.f);
     return a < 0.5f ? __builtin_fmaf(x * s, p, x) : far;
 }
-__device__ __forceinline__ void values4(float (&v)[4], const f32x4 scaled, const Columns4& c, bool biased, int act) {
+__device__ __forceinline__ void values4(float (&v)[4], const f32x4 scaled, const Columns4& c, bool biased, int act, int dtype) {
 #pragma clang fp contract(off)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -563,6 +564,9 @@ __device__ __forceinline__ void values4(float (&v)[4], const f32x4 scaled, const
     if (act == ACT_RELU) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];       // keeps NaN
+    } else if (act == ACT_TANH && dtype == F_FP32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = tanhf(v[i]);
     } else if (act == ACT_TANH) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = tanh_of(v[i]);
@@ -576,7 +580,7 @@ __device__ __forceinline__ void store_values4(void* out, long long at, int dtype
 __device__ __forceinline__ void finish4(const LinearInt8Args& a, int m, int n, const f32x4 scaled, const Columns4& c) {
     if (m >= a.M || n >= a.N) return;
     float v[4];
-    values4(v, scaled, c, a.bias != nullptr, a.act);
+    values4(v, scaled, c, a.bias != nullptr, a.act, a.dtype);
     store_values4(a.out, (long long)m * a.ld_out + n, a.dtype, v, a.N - n);
 }
 
@@ -1157,7 +1161,7 @@ __device__ __forceinline__ void mlp3_rows(const Mlp3Int8Args& a, signed char* co
             Columns4 cc;
             *reinterpret_cast<f32x4*>(cc.scale) = *reinterpret_cast<const f32x4*>(cols + col);
             *reinterpret_cast<f32x4*>(cc.bias) = *reinterpret_cast<const f32x4*>(cols + 64 + col);
-            values4(y, scaled4(sum, sr), cc, biased, act);
+            values4(y, scaled4(sum, sr), cc, biased, act, a.dtype);
             if (layer == 2) {
                 if (m0 + r < a.M && n < N) store_values4(a.out, (long long)(m0 + r) * a.ld_out + n, a.dtype, y, N - n);
             } else {

@@ -140,3 +140,23 @@ def test_both_devices_make_the_same_codes(dtype):
     x = (_randn(300, 700, seed=1) * torch.exp(20 * _randn(300, 1, seed=2)).clamp(1e-3, 1e3)).to(dtype)
     for a, b in zip(ops.quantize_rows(x), ops.quantize_rows(x.cuda())):
         assert torch.equal(a, b.cpu())
+
+
+# ------------------------------------------------------------------------------------------------------ tanh in 32 bits
+@pytest.mark.gpu
+def test_tanh_of_fp32_results_is_within_two_units_of_the_last_place():
+    """One column: the sum times its scale is the argument itself, so all of the error is the function's.  Division and
+    exponential of full precision leave at most 1.4 units; two are allowed, and as much through the policy's last layer."""
+    v = torch.cat([torch.linspace(0.25, 1.25, 1 << 20), torch.linspace(1.25, 10, 1 << 18)]).cuda()
+    v = torch.cat([v, -v])
+    one = torch.ones(v.numel(), 1, dtype=torch.int8, device="cuda")
+    want = torch.tanh(v.double())
+    unit = torch.ldexp(torch.ones_like(want), torch.frexp(want).exponent - 24)
+    y = ops.linear_int8(one, v, one[:1], torch.ones(1, device="cuda"), None, "tanh")[:, 0]
+    assert torch.all((y.double() - want).abs() <= 2 * unit)
+    x = v[: 1 << 20: 16, None].clone()
+    eye = (torch.ones(1, 1, dtype=torch.int8, device="cuda"), torch.ones(1, device="cuda"), None)
+    y = ops.mlp3_int8(x, (eye, eye, eye), "tanh")[:, 0]
+    h = ops.mlp3_int8(x, (eye, eye, eye))[:, 0].double()
+    unit = torch.ldexp(torch.ones_like(h), torch.frexp(torch.tanh(h)).exponent - 24)
+    assert torch.all((y.double() - torch.tanh(h)).abs() <= 2 * unit)
