@@ -34,6 +34,8 @@ from .gpu_actor import PackedActor32
 class DeviceRollout:
     def __init__(self, cfg: Dict, env, replay, device="cuda", segment: int = 32, seed: int = 0,
                  explore: bool = True, use_graph: bool = True, fuse_noise: bool = True):
+        if cfg.get("policy_precision", "fp32") != "fp32":
+            raise ValueError("device explorers act in fp32: policy_precision must be 'fp32' where they run")
         self.cfg, self.env, self.replay = cfg, env, replay
         self.device = torch.device(device)
         self.E, self.T = env.E, int(segment)

@@ -111,8 +111,10 @@ EXTENSION_DEFAULTS: Dict[str, Any] = {
                                      # MFMA, fused row-local pipeline, tracks eager PyTorch to rounding) | "bf16"
                                      # (opt-in: the same pipeline with bf16 MFMA operands; fp32 master weights, Adam,
                                      # logits and loss)
-    "policy_precision": "fp32",      # agents that act on a GPU: "fp32" | "int8" (weights quantised per output channel, states and
-                                     # hidden activations per row; ops/int8.py).  Training stays as compute_dtype says
+    "policy_precision": "fp32",      # agents that act on a GPU (exploiter_device, agent_device): "fp32" | "int8" (weights quantised
+                                     # per output channel, states and hidden activations per row; ops/int8.py).  Agents on
+                                     # the CPU act in fp32; "int8" is refused where no agent acts on a GPU and beside device
+                                     # explorers (gpu_rollout_envs), whose policy is fp32.  Training stays as compute_dtype says
     "use_hip_graph": True,           # replay the whole update as one captured HIP graph
     "fused_learner": "auto",         # "auto": HIP kernels on cuda, torch ops on cpu; "torch": force eager torch;
                                      # "layers": the fp32 kernels with one launch per layer (any shape)
@@ -321,6 +323,11 @@ def finalize_config(raw: Dict[str, Any]) -> Dict[str, Any]:
         cfg["replay_device"] = "hbm" if dev.startswith("cuda") else "host"
     if cfg["exploiter_device"] is None:
         cfg["exploiter_device"] = dev
+    if cfg["policy_precision"] == "int8":
+        need(cfg["gpu_rollout_envs"] == 0, "policy_precision 'int8' does not reach device explorers (gpu_rollout_envs > 0), "
+                                           "which act in fp32")
+        need(str(cfg["exploiter_device"]).startswith("cuda") or str(cfg["agent_device"]).startswith("cuda"),
+             "policy_precision 'int8' needs an agent that acts on a GPU (exploiter_device or agent_device: cuda)")
     if cfg["learner_devices"] is None:
         cfg["learner_devices"] = list(range(cfg["num_learners"]))
     if cfg["min_replay_size"] is None:

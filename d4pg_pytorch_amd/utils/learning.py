@@ -60,6 +60,8 @@ class GreedyEvaluator:
     def __init__(self, cfg: Dict, envs: int, device, seed: int):
         from ..actors.gpu_actor import PackedActor32
         from ..envs.device_envs import make_device_env
+        if cfg.get("policy_precision", "fp32") != "fp32":
+            raise ValueError("the greedy policy is evaluated in fp32: policy_precision must be 'fp32' here")
         self.device = torch.device(device)
         self.env = make_device_env(dict(cfg, env_backend="native"), envs, device, seed)      # (never gym: evaluation on the device)
         S, A = self.env.state_dim, self.env.action_dim

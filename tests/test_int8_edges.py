@@ -160,3 +160,20 @@ def test_tanh_of_fp32_results_is_within_two_units_of_the_last_place():
     h = ops.mlp3_int8(x, (eye, eye, eye))[:, 0].double()
     unit = torch.ldexp(torch.ones_like(h), torch.frexp(torch.tanh(h)).exponent - 24)
     assert torch.all((y.double() - torch.tanh(h)).abs() <= 2 * unit)
+
+
+# ------------------------------------------------------------------------------------ where the agents' key does not reach
+def test_the_precision_key_is_refused_where_it_would_do_nothing():
+    from d4pg_pytorch_amd.actors.gpu_rollout import DeviceRollout
+    from d4pg_pytorch_amd.config import ConfigError, default_config
+    from d4pg_pytorch_amd.utils.learning import GreedyEvaluator
+    for kw in (dict(gpu_rollout_envs=64), dict(device="cpu"), dict(device="cpu", agent_device="cpu"), dict(exploiter_device="cpu")):
+        with pytest.raises(ConfigError, match="policy_precision"):
+            default_config(env="Pendulum-v0", policy_precision="int8", **kw)
+    for kw in (dict(), dict(device="cpu", agent_device="cuda"), dict(exploiter_device="cuda:0", agent_device="cpu")):
+        assert default_config(env="Pendulum-v0", policy_precision="int8", **kw)["policy_precision"] == "int8"
+    cfg = dict(default_config(env="Pendulum-v0"), policy_precision="int8")
+    with pytest.raises(ValueError, match="policy_precision"):
+        DeviceRollout(cfg, None, None)
+    with pytest.raises(ValueError, match="policy_precision"):
+        GreedyEvaluator(cfg, 4, "cpu", 1)
