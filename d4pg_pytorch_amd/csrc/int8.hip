@@ -21,6 +21,15 @@
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
+// A launch and its own status: an error that another call has left pending is neither taken for this one's nor cleared.
+template <typename A>
+static int enqueue(void (*kernel)(A), dim3 grid, int block, int lds, hipStream_t stream, A a) {
+    void* args[] = {&a};
+    const hipError_t rc = hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, dim3(block), args, lds, stream);
+    if (rc != hipSuccess) (void)hipGetLastError();         // reported by the return value
+    return (int)rc;
+}
+
 // ---------------------------------------------------------------------------------------------------------------
 // floating rows -> codes
 // ---------------------------------------------------------------------------------------------------------------
@@ -395,7 +404,7 @@ __global__ __launch_bounds__(1024) void quant_long_rows_kernel(const QuantRowsAr
 
 // A launch holds fewer than 2^32 threads: more rows than that are several launches.
 template <typename F>
-static void launch_row_ranges(QuantRowsArgs a, long long element, int block, int rows_per_block, F launch) {
+static int launch_row_ranges(QuantRowsArgs a, long long element, int block, int rows_per_block, F launch) {
     const long long most = (0xffffffffll / block) * rows_per_block, M = a.M;
     for (long long done = 0; done < M; done += most) {
         QuantRowsArgs part = a;
@@ -404,39 +413,38 @@ static void launch_row_ranges(QuantRowsArgs a, long long element, int block, int
         if (a.residual != nullptr) part.residual = (const char*)a.residual + done * a.ld_r * element;
         if (a.h != nullptr) part.h = (char*)a.h + done * a.ld_h * element;
         part.q = a.q + done * a.ld_q, part.scale = a.scale + done;
-        launch(part, dim3((unsigned)((part.M + rows_per_block - 1) / rows_per_block)));
+        const int rc = launch(part, dim3((unsigned)((part.M + rows_per_block - 1) / rows_per_block)));
+        if (rc != 0) return rc;
     }
+    return 0;
 }
 template <typename T, int G, int V>
-static void launch_rows(const QuantRowsArgs& a, hipStream_t stream) {
+static int launch_rows(const QuantRowsArgs& a, hipStream_t stream) {
     constexpr int BLOCK = G < 256 ? 256 : G;
-    launch_row_ranges(a, sizeof(T), BLOCK, BLOCK / G, [&](const QuantRowsArgs& part, dim3 grid) {
-        if (a.norm) hipLaunchKernelGGL((quant_rows_kernel<T, G, V, true>), grid, dim3(BLOCK), 0, stream, part);
-        else hipLaunchKernelGGL((quant_rows_kernel<T, G, V, false>), grid, dim3(BLOCK), 0, stream, part);
+    return launch_row_ranges(a, sizeof(T), BLOCK, BLOCK / G, [&](const QuantRowsArgs& part, dim3 grid) {
+        return enqueue(a.norm ? quant_rows_kernel<T, G, V, true> : quant_rows_kernel<T, G, V, false>, grid, BLOCK, 0, stream, part);
     });
 }
 template <typename T>
-static void launch_rows_of(const QuantRowsArgs& a, hipStream_t stream) {
+static int launch_rows_of(const QuantRowsArgs& a, hipStream_t stream) {
     // c: chunks of 8 a row needs.  Short rows share a wave, long ones take as few threads as hold them in 4 chunks each (8 from
     // 8192 columns on); where the rows are fewer than the CUs, 1024 threads answer sooner than 256.  Measured: 65536 x 100 fp32
     // 7.1 us, 18.5 with a wave
     // a row; 1 x 16384 bf16 with a residual 5.0 us, 8.8 with 256 threads.
     const long long c = a.ld_q >> 3;
-    if (c <= 16) launch_rows<T, 16, 1>(a, stream);
-    else if (c <= 32) launch_rows<T, 16, 2>(a, stream);
-    else if (c <= 64) launch_rows<T, 64, 1>(a, stream);
-    else if (c <= 128) launch_rows<T, 64, 2>(a, stream);
-    else if (c <= 256) launch_rows<T, 64, 4>(a, stream);
-    else if (c <= 512) launch_rows<T, 256, 2>(a, stream);
-    else if (c <= 2048 && a.M <= 256) launch_rows<T, 1024, 2>(a, stream);
-    else if (c <= 1024) launch_rows<T, 256, 4>(a, stream);
-    else if (c <= 2048) launch_rows<T, 256, 8>(a, stream);
-    else if (c <= 4096) launch_rows<T, 1024, 4>(a, stream);
-    else
-        launch_row_ranges(a, sizeof(T), 1024, 1, [&](const QuantRowsArgs& part, dim3 grid) {
-            if (a.norm) hipLaunchKernelGGL((quant_long_rows_kernel<T, true>), grid, dim3(1024), 0, stream, part);
-            else hipLaunchKernelGGL((quant_long_rows_kernel<T, false>), grid, dim3(1024), 0, stream, part);
-        });
+    if (c <= 16) return launch_rows<T, 16, 1>(a, stream);
+    else if (c <= 32) return launch_rows<T, 16, 2>(a, stream);
+    else if (c <= 64) return launch_rows<T, 64, 1>(a, stream);
+    else if (c <= 128) return launch_rows<T, 64, 2>(a, stream);
+    else if (c <= 256) return launch_rows<T, 64, 4>(a, stream);
+    else if (c <= 512) return launch_rows<T, 256, 2>(a, stream);
+    else if (c <= 2048 && a.M <= 256) return launch_rows<T, 1024, 2>(a, stream);
+    else if (c <= 1024) return launch_rows<T, 256, 4>(a, stream);
+    else if (c <= 2048) return launch_rows<T, 256, 8>(a, stream);
+    else if (c <= 4096) return launch_rows<T, 1024, 4>(a, stream);
+    return launch_row_ranges(a, sizeof(T), 1024, 1, [&](const QuantRowsArgs& part, dim3 grid) {
+        return enqueue(a.norm ? quant_long_rows_kernel<T, true> : quant_long_rows_kernel<T, false>, grid, 1024, 0, stream, part);
+    });
 }
 
 D4PG_API int d4pg_quant_rows(const QuantRowsArgs* a, hipStream_t stream) {
@@ -445,11 +453,10 @@ D4PG_API int d4pg_quant_rows(const QuantRowsArgs* a, hipStream_t stream) {
     if ((a->ld_q & 15) || a->ld_q < a->K || a->ld_q >= a->K + 16 || ((uintptr_t)a->q & 15)) return -3;
     if (a->wdtype != F_NONE && (a->weight == nullptr || a->wdtype < 0 || a->wdtype > F_FP16)) return -4;
     if (!a->norm && (a->residual != nullptr || a->weight != nullptr || a->h != nullptr)) return -5;
-    if (a->dtype == F_FP32) launch_rows_of<float>(*a, stream);
-    else if (a->dtype == F_BF16) launch_rows_of<__bf16>(*a, stream);
-    else if (a->dtype == F_FP16) launch_rows_of<_Float16>(*a, stream);
-    else return -6;
-    return (int)hipGetLastError();
+    if (a->dtype == F_FP32) return launch_rows_of<float>(*a, stream);
+    if (a->dtype == F_BF16) return launch_rows_of<__bf16>(*a, stream);
+    if (a->dtype == F_FP16) return launch_rows_of<_Float16>(*a, stream);
+    return -6;
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -493,12 +500,12 @@ D4PG_API int d4pg_dequant_rows(DequantRowsArgs* a, hipStream_t stream) {
         part.q = a->q + done * a->ld_q, part.scale = a->scale + done, part.out = (char*)a->out + done * a->K * bytes;
         // few long rows: several workgroups each
         const long long blocks = (part.M + rpb - 1) / rpb, pieces = (a->K + 2047) / 2048, spread = 1024 / blocks + 1;
-        const dim3 grid((unsigned)blocks, (unsigned)(spread < pieces ? spread : pieces)), block(256);
-        if (a->dtype == F_FP32) hipLaunchKernelGGL(dequant_rows_kernel<float>, grid, block, 0, stream, part);
-        else if (a->dtype == F_BF16) hipLaunchKernelGGL(dequant_rows_kernel<__bf16>, grid, block, 0, stream, part);
-        else hipLaunchKernelGGL(dequant_rows_kernel<_Float16>, grid, block, 0, stream, part);
+        const dim3 grid((unsigned)blocks, (unsigned)(spread < pieces ? spread : pieces));
+        const int rc = enqueue(a->dtype == F_FP32 ? dequant_rows_kernel<float> : a->dtype == F_BF16 ? dequant_rows_kernel<__bf16> : dequant_rows_kernel<_Float16>,
+                               grid, 256, 0, stream, part);
+        if (rc != 0) return rc;
     }
-    return (int)hipGetLastError();
+    return 0;
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -673,8 +680,7 @@ template <int MT, int NT, int WAVES, int U>
 static int launch_linear_rows(const LinearInt8Args& a, hipStream_t stream) {
     const long long tiles = (long long)((a.M + 16 * MT - 1) / (16 * MT)) * ((a.N + 16 * NT - 1) / (16 * NT));
     if (tiles * (64 * WAVES) > 0xffffffffll) return TOO_MANY;
-    hipLaunchKernelGGL((linear_int8_rows_kernel<MT, NT, WAVES, U>), dim3((unsigned)tiles), dim3(64 * WAVES), 0, stream, a);
-    return (int)hipGetLastError();
+    return enqueue(linear_int8_rows_kernel<MT, NT, WAVES, U>, dim3((unsigned)tiles), 64 * WAVES, 0, stream, a);
 }
 
 // Many rows: a workgroup of WM x WN waves makes a tile of BM = 32 MI WM rows x BN = 32 NI WN columns, a wave 32 MI x 32 NI
@@ -837,8 +843,7 @@ static int launch_linear_tiles(const LinearInt8Args& a, hipStream_t stream) {
     constexpr int LDS = TILES > STAGE ? TILES : STAGE;
     const long long tiles = (long long)((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN);
     if (tiles * (64 * WM * WN * KW) > 0xffffffffll) return TOO_MANY;
-    hipLaunchKernelGGL((linear_int8_tiles_kernel<MI, NI, WM, WN, KW, S>), dim3((unsigned)tiles), dim3(64 * WM * WN * KW), LDS, stream, a);
-    return (int)hipGetLastError();
+    return enqueue(linear_int8_tiles_kernel<MI, NI, WM, WN, KW, S>, dim3((unsigned)tiles), 64 * WM * WN * KW, LDS, stream, a);
 }
 
 // Which kernel.  Tiles are taken from the largest size that still gives most of the 256 CUs one and is not more than twice as
@@ -1234,17 +1239,16 @@ __global__ __launch_bounds__(64 * MLP_WAVES) void mlp3_int8_kernel(const Mlp3Int
     mlp3_rows<TPW, MT>(a, net);
 }
 
-// 1: does not fit the LDS
+// NOT_TAKEN: does not fit the LDS
 template <int TPW, int MT>
 static int launch_mlp3(Mlp3Int8Args& a, int few, hipStream_t stream) {
     a.split = few * MT * 256;
     const int lds = MLP_WAVES * (mlp_ring(MT) * 1024 + 512) + 16 * MT * a.pitch + 4 * a.split + 3 * 16 * MT * 4;
-    if (lds > 160 * 1024) return 1;
-    hipLaunchKernelGGL((mlp3_int8_kernel<TPW, MT>), dim3((unsigned)((a.M + 16 * MT - 1) / (16 * MT))), dim3(64 * MLP_WAVES), lds, stream, a);
-    return (int)hipGetLastError();
+    if (lds > 160 * 1024) return NOT_TAKEN;
+    return enqueue(mlp3_int8_kernel<TPW, MT>, dim3((unsigned)((a.M + 16 * MT - 1) / (16 * MT))), 64 * MLP_WAVES, lds, stream, a);
 }
 
-// 0: enqueued; 1: outside this kernel's range (nothing was enqueued); < 0: bad arguments.
+// NOT_TAKEN: outside this kernel's range.
 D4PG_API int d4pg_mlp3_int8(Mlp3Int8Args* a, hipStream_t stream) {
     if (a->M < 1 || a->x == nullptr || a->out == nullptr || a->ld_out < a->width[3]) return -1;
     if (a->dtype < F_FP32 || a->dtype > F_FP16 || a->xdtype < F_FP32 || a->xdtype > F_FP16) return -6;
@@ -1258,12 +1262,12 @@ D4PG_API int d4pg_mlp3_int8(Mlp3Int8Args* a, hipStream_t stream) {
         const long long kp = (a->width[i] + 15) & ~15;
         if (a->w[i] == nullptr || a->wscale[i] == nullptr) return -2;
         if (((uintptr_t)a->w[i] & 15) || (a->width[i + 1] > 1 && ((a->ld_w[i] & 15) || a->ld_w[i] < kp))) return -3;
-        if (a->ld_w[i] >= 1 << 20) return 1;        // offsets inside a matrix are 32-bit
+        if (a->ld_w[i] >= 1 << 20) return NOT_TAKEN;        // offsets inside a matrix are 32-bit
         const int tiles = (a->width[i + 1] + 15) / 16;
         if (tiles > wide_out) wide_out = tiles;
         if (tiles <= MLP_WAVES / 2 && tiles > few) few = tiles;
     }
-    if (widest > 2048 || wide_out > 64 || a->M > 1 << 25) return 1;       // (2^25 rows: 2^31 threads)
+    if (widest > 2048 || wide_out > 64 || a->M > 1 << 25) return NOT_TAKEN;       // (2^25 rows: 2^31 threads)
     a->pitch = ((widest + 63) & ~63) + 16;
     const bool two = a->M > 4096;                // 32 rows a workgroup, so that one round of workgroups holds them longer
     if (wide_out <= 16) return two ? launch_mlp3<1, 2>(*a, few, stream) : launch_mlp3<1, 1>(*a, few, stream);

@@ -4,6 +4,8 @@
 
 enum { F_FP32 = 0, F_BF16 = 1, F_FP16 = 2, F_NONE = -1 };
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_TANH = 2 };
+// What the entries return: 0, enqueued; a hipError_t (positive), the launch's own; negative, refused and nothing enqueued.
+enum { NOT_TAKEN = -100 };         // mlp3: good arguments, outside the one launch's range
 
 // floating rows -> codes
 struct QuantRowsArgs {

@@ -3,7 +3,8 @@
 // At the sizes one state or one token has, an operator's kernel runs for 2 - 5 us and the call around it decides: the
 // checks and the descriptor cost 5 us in Python, 0.5 us here.  A function of this module takes exactly the plain case -
 // dense tensors on the current device, types, shapes and strides as the kernels read them - and returns None for anything
-// else: ops/int8.py then converts layouts, or says what is wrong.  It decides nothing by itself.
+// else: ops/int8.py then converts layouts, or says what is wrong.  It decides nothing by itself.  A launch that HIP refuses
+// raises here: the work of an entry that returned a hipError_t is not tried again.
 #include <Python.h>
 #include <ATen/ATen.h>
 #include <c10/hip/HIPFunctions.h>
@@ -67,6 +68,12 @@ hipStream_t stream(int dev) { return c10::hip::getCurrentHIPStream(dev).stream()
 float* f32(const Tensor& t) { return static_cast<float*>(t.data_ptr()); }
 const float* f32c(const Tensor& t) { return static_cast<const float*>(t.const_data_ptr()); }
 
+// 0: enqueued.  false: refused by the entry's own checks.
+bool enqueued(int rc, const char* what) {
+    TORCH_CHECK(rc <= 0, what, " failed with code ", rc);
+    return rc == 0;
+}
+
 struct Weights {
     const signed char* w;
     const float *scale, *bias;
@@ -98,7 +105,7 @@ PyObject* linear(PyObject*, PyObject* const* o, Py_ssize_t n) {
     a.q = static_cast<const signed char*>(q->const_data_ptr()), a.scale = f32c(*s), a.w = l.w, a.wscale = l.scale, a.bias = l.bias;
     a.out = out.data_ptr(), a.ld_w = l.ld, a.ld_out = l.N;
     a.M = (int)q->size(0), a.N = (int)l.N, a.K = (int)q->size(1), a.act = (int)act, a.dtype = (int)dtype;
-    if (linear_int8(&a, stream(dev)) != 0) Py_RETURN_NONE;
+    if (!enqueued(linear_int8(&a, stream(dev)), "d4pg_linear_int8")) Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(out));
     END_HANDLE_TH_ERRORS
 }
@@ -136,7 +143,7 @@ PyObject* quantize(PyObject*, PyObject* const* o, Py_ssize_t n) {
     }
     Tensor q = new_codes(a.M, a.K, *x), scale = at::empty({a.M}, x->options().dtype(at::kFloat));
     a.q = static_cast<signed char*>(q.data_ptr()), a.scale = f32(scale);
-    if (quant_rows(&a, stream(dev)) != 0) Py_RETURN_NONE;
+    if (!enqueued(quant_rows(&a, stream(dev)), "d4pg_quant_rows")) Py_RETURN_NONE;
     PyObject* t = PyTuple_New(n == 4 ? 3 : 2);
     if (!t) return nullptr;
     PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(std::move(q)));
@@ -162,7 +169,7 @@ PyObject* dequantize(PyObject*, PyObject* const* o, Py_ssize_t n) {
     DequantRowsArgs a = {};
     a.q = static_cast<const signed char*>(q->const_data_ptr()), a.scale = f32c(*s), a.out = out.data_ptr();
     a.M = q->size(0), a.K = q->size(1), a.ld_q = q->stride(0), a.dtype = (int)dtype;
-    if (dequant_rows(&a, stream(dev)) != 0) Py_RETURN_NONE;
+    if (!enqueued(dequant_rows(&a, stream(dev)), "d4pg_dequant_rows")) Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(out));
     END_HANDLE_TH_ERRORS
 }
@@ -174,12 +181,12 @@ Tensor coded_layer(const Tensor& x, const Weights& l, int act, int dtype, hipStr
     QuantRowsArgs r = {};
     r.x = x.const_data_ptr(), r.q = static_cast<signed char*>(q.data_ptr()), r.scale = f32(scale);
     r.M = M, r.K = K, r.ld_x = x.stride(0), r.ld_q = padded(K), r.dtype = float_code(x.scalar_type()), r.wdtype = F_NONE;
-    if (quant_rows(&r, s) != 0) return Tensor();
+    if (!enqueued(quant_rows(&r, s), "d4pg_quant_rows")) return Tensor();
     Tensor out = at::empty({M, l.N}, x.options().dtype(float_type(dtype)));
     LinearInt8Args a = {};
     a.q = r.q, a.scale = r.scale, a.w = l.w, a.wscale = l.scale, a.bias = l.bias, a.out = out.data_ptr();
     a.ld_q = r.ld_q, a.ld_w = l.ld, a.ld_out = l.N, a.M = (int)M, a.N = (int)l.N, a.K = (int)K, a.act = act, a.dtype = dtype;
-    return linear_int8(&a, s) == 0 ? out : Tensor();
+    return enqueued(linear_int8(&a, s), "d4pg_linear_int8") ? out : Tensor();
 }
 
 // mlp3(x, weight, weight_scale, bias, ... three times, activation code, type code)
@@ -207,11 +214,11 @@ PyObject* mlp3(PyObject*, PyObject* const* o, Py_ssize_t n) {
     a.xdtype = float_code(x->scalar_type()), a.dtype = (int)dtype, a.act = (int)act;
     const hipStream_t s = stream(dev);
     const int rc = mlp3_int8(&a, s);
-    if (rc == 1) {               // wider than its LDS: a launch a step
+    if (rc == NOT_TAKEN) {       // wider than its LDS: a launch a step
         out = *x;
         for (int i = 0; i < 3 && out.defined(); ++i) out = coded_layer(out, l[i], i < 2 ? ACT_RELU : (int)act, i < 2 ? F_FP32 : (int)dtype, s);
         if (!out.defined()) Py_RETURN_NONE;
-    } else if (rc != 0) {
+    } else if (!enqueued(rc, "d4pg_mlp3_int8")) {
         Py_RETURN_NONE;
     }
     return THPVariable_Wrap(std::move(out));

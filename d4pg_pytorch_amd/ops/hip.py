@@ -31,6 +31,7 @@ GEMM_NT, GEMM_NN, GEMM_TN = 0, 1, 2
 EPI_NONE, EPI_RELU, EPI_TANH, EPI_MUL_RELU_MASK, EPI_MUL_TANH_GRAD = 0, 1, 2, 3, 4
 F_NONE, F_FP32, F_BF16, F_FP16 = -1, 0, 1, 2           # floating types of csrc/int8.hip
 ACT_NONE, ACT_RELU, ACT_TANH = 0, 1, 2
+NOT_TAKEN = -100                                       # d4pg_mlp3_int8: outside the one launch's range
 MAX_GROUP = 6
 MAXL = 6
 

@@ -340,7 +340,7 @@ def _mlp3_fused(x: torch.Tensor, layers, final: str, dtype: torch.dtype, dt: int
         a.x, a.ld_x, a.out, a.ld_out, a.M = x2.data_ptr(), x2.stride(0), out.data_ptr(), K, M
         a.xdtype, a.dtype, a.act = xdt, dt, _ACTS[final]
         rc = H.launch_on("d4pg_mlp3_int8", a, device.index)
-        if rc == 1:              # too wide for one workgroup's LDS
+        if rc == H.NOT_TAKEN:    # too wide for one workgroup's LDS
             return None
         if rc:
             H._check(rc, "d4pg_mlp3_int8")

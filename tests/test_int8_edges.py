@@ -177,3 +177,87 @@ def test_the_precision_key_is_refused_where_it_would_do_nothing():
         DeviceRollout(cfg, None, None)
     with pytest.raises(ValueError, match="policy_precision"):
         GreedyEvaluator(cfg, 4, "cpu", 1)
+
+
+# ---------------------------------------------------------------------------------------------------- what entries return
+def _policy(M, dims, device="cuda"):
+    """A launch descriptor of ``mlp3_int8`` and what it points to."""
+    from d4pg_pytorch_amd.ops import hip as H
+    a = H.Mlp3Int8Args()
+    x, out = _randn(M, dims[0], seed=1).to(device), torch.empty(M, dims[3], device=device)
+    layers = [(*ops.quantize_rows(_randn(dims[i + 1], dims[i], seed=i).to(device)), _randn(dims[i + 1], seed=i).to(device)) for i in range(3)]
+    for i, (w, s, b) in enumerate(layers):
+        a.w[i], a.wscale[i], a.bias[i], a.ld_w[i] = w.data_ptr(), s.data_ptr(), b.data_ptr(), w.stride(0)
+    a.x, a.ld_x, a.out, a.ld_out, a.M, a.width[:] = x.data_ptr(), dims[0], out.data_ptr(), dims[3], M, dims
+    return a, x, layers, out
+
+
+def test_a_policy_outside_the_one_launch_is_told_from_an_error():
+    """The code for it is no ``hipError_t`` (those are positive); nothing is launched, so no GPU is needed."""
+    import ctypes as C
+
+    from d4pg_pytorch_amd.ops import hip as H
+    for dims in ([2100, 64, 64, 2], [16, 1025, 64, 2], [16, 64, 64, 1030], [2000, 1024, 1024, 120]):
+        a, *held = _policy(3, dims, "cpu")
+        assert H.lib().d4pg_mlp3_int8(C.byref(a), None) == H.NOT_TAKEN < 0, dims
+
+
+@pytest.mark.gpu
+def test_an_error_left_by_another_call_is_not_taken_for_an_operators_own():
+    import ctypes as C
+    import os
+
+    from d4pg_pytorch_amd import build
+    from d4pg_pytorch_amd.ops import hip as H
+    hip = C.CDLL(os.path.join(build.torch_lib_dir(), "libamdhip64.so"))
+    a, x, layers, out = _policy(5, [24, 64, 64, 3])
+    want = ops.mlp3_int8(x, layers)
+    q, s = ops.quantize_rows(x)
+    w, ws, _ = layers[0]
+    buf, y, v = torch.empty(5, 32, dtype=torch.int8, device="cuda"), torch.empty(5, 64, device="cuda"), torch.empty(5, 24, device="cuda")
+    codes = H.QuantRowsArgs(x.data_ptr(), None, None, None, buf.data_ptr(), s.data_ptr(), 5, 24, 24, 0, 0, 32, 0, H.F_NONE, 0, 0.0)
+    product = H.LinearInt8Args(q.data_ptr(), s.data_ptr(), w.data_ptr(), ws.data_ptr(), None, y.data_ptr(), 32, 32, 64, 5, 64, 24, 0, 0, 0)
+    values = H.DequantRowsArgs(q.data_ptr(), s.data_ptr(), v.data_ptr(), 5, 24, 32, 0, 0)
+    torch.cuda.synchronize()
+    got = {}
+    for name, args in (("d4pg_mlp3_int8", a), ("d4pg_quant_rows", codes), ("d4pg_linear_int8", product), ("d4pg_dequant_rows", values)):
+        assert hip.hipGetDevice(None) == 1                # hipErrorInvalidValue: refused on the host, left pending
+        got[name] = H.launch_on(name, args, 0)
+        hip.hipGetLastError()
+    assert got == dict.fromkeys(got, 0)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(buf[:, :24], q)
+    assert torch.equal(y, ops.linear_int8(q, s, w, ws)) and torch.equal(v, ops.dequantize_rows(q, s))
+
+
+@pytest.mark.gpu
+def test_a_launch_that_hip_refuses_raises_and_is_not_tried_again():
+    """Entries that return a ``hipError_t`` (nothing reaches the GPU here) in the place of the library's."""
+    import ctypes as C
+
+    from d4pg_pytorch_amd.ops import hip as H
+    x = _randn(4, 20, seed=1).cuda()
+    q, s = ops.quantize_rows(x)
+    layers = [(*ops.quantize_rows(_randn(4, k, seed=k).cuda()), None) for k in (20, 4, 4)]
+    calls, codes = [], [0]
+
+    @C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_void_p)
+    def entry(args, stream):
+        calls.append(args)
+        return codes[0]
+
+    binding = H.int8_binding()
+    real = [C.cast(getattr(H.lib(), name), C.c_void_p).value for name in ("d4pg_quant_rows", "d4pg_dequant_rows", "d4pg_linear_int8", "d4pg_mlp3_int8")]
+    try:
+        binding.bind(*[C.cast(entry, C.c_void_p).value] * 4)
+        for code in (1, 719):
+            codes[0] = code
+            for call in (lambda: ops.quantize_rows(x), lambda: ops.add_rms_norm_int8(x), lambda: ops.dequantize_rows(q, s),
+                         lambda: ops.linear_int8(q, s, q, s), lambda: ops.mlp3_int8(x, layers)):
+                calls.clear()
+                with pytest.raises(RuntimeError, match=f"failed with code {code}"):
+                    call()
+                assert len(calls) == 1
+    finally:
+        binding.bind(*real)
+    assert torch.equal(ops.quantize_rows(x)[0], q)
