@@ -402,10 +402,15 @@ __global__ __launch_bounds__(1024) void quant_long_rows_kernel(const QuantRowsAr
     if (threadIdx.x == 0) a.scale[row] = code.scale;
 }
 
-// A launch holds fewer than 2^32 threads: more rows than that are several launches.
+// A launch holds fewer than 2^32 threads: more rows than that are several launches.  The entries whose names end in _in take
+// the limit as an argument (1024, a workgroup, at least; the product's: what 16 rows need), so that what follows the first
+// launch can be had with few rows.
+constexpr long long LAUNCH_THREADS = 0xffffffffll;
+static bool good_limit(long long threads) { return threads >= 1024 && threads <= LAUNCH_THREADS; }
+
 template <typename F>
-static int launch_row_ranges(QuantRowsArgs a, long long element, int block, int rows_per_block, F launch) {
-    const long long most = (0xffffffffll / block) * rows_per_block, M = a.M;
+static int launch_row_ranges(QuantRowsArgs a, long long threads, long long element, int block, int rows_per_block, F launch) {
+    const long long most = (threads / block) * rows_per_block, M = a.M;
     for (long long done = 0; done < M; done += most) {
         QuantRowsArgs part = a;
         part.M = M - done < most ? M - done : most;
@@ -419,45 +424,47 @@ static int launch_row_ranges(QuantRowsArgs a, long long element, int block, int 
     return 0;
 }
 template <typename T, int G, int V>
-static int launch_rows(const QuantRowsArgs& a, hipStream_t stream) {
+static int launch_rows(const QuantRowsArgs& a, long long threads, hipStream_t stream) {
     constexpr int BLOCK = G < 256 ? 256 : G;
-    return launch_row_ranges(a, sizeof(T), BLOCK, BLOCK / G, [&](const QuantRowsArgs& part, dim3 grid) {
+    return launch_row_ranges(a, threads, sizeof(T), BLOCK, BLOCK / G, [&](const QuantRowsArgs& part, dim3 grid) {
         return enqueue(a.norm ? quant_rows_kernel<T, G, V, true> : quant_rows_kernel<T, G, V, false>, grid, BLOCK, 0, stream, part);
     });
 }
 template <typename T>
-static int launch_rows_of(const QuantRowsArgs& a, hipStream_t stream) {
+static int launch_rows_of(const QuantRowsArgs& a, long long threads, hipStream_t stream) {
     // c: chunks of 8 a row needs.  Short rows share a wave, long ones take as few threads as hold them in 4 chunks each (8 from
     // 8192 columns on); where the rows are fewer than the CUs, 1024 threads answer sooner than 256.  Measured: 65536 x 100 fp32
     // 7.1 us, 18.5 with a wave
     // a row; 1 x 16384 bf16 with a residual 5.0 us, 8.8 with 256 threads.
     const long long c = a.ld_q >> 3;
-    if (c <= 16) return launch_rows<T, 16, 1>(a, stream);
-    else if (c <= 32) return launch_rows<T, 16, 2>(a, stream);
-    else if (c <= 64) return launch_rows<T, 64, 1>(a, stream);
-    else if (c <= 128) return launch_rows<T, 64, 2>(a, stream);
-    else if (c <= 256) return launch_rows<T, 64, 4>(a, stream);
-    else if (c <= 512) return launch_rows<T, 256, 2>(a, stream);
-    else if (c <= 2048 && a.M <= 256) return launch_rows<T, 1024, 2>(a, stream);
-    else if (c <= 1024) return launch_rows<T, 256, 4>(a, stream);
-    else if (c <= 2048) return launch_rows<T, 256, 8>(a, stream);
-    else if (c <= 4096) return launch_rows<T, 1024, 4>(a, stream);
-    return launch_row_ranges(a, sizeof(T), 1024, 1, [&](const QuantRowsArgs& part, dim3 grid) {
+    if (c <= 16) return launch_rows<T, 16, 1>(a, threads, stream);
+    if (c <= 32) return launch_rows<T, 16, 2>(a, threads, stream);
+    if (c <= 64) return launch_rows<T, 64, 1>(a, threads, stream);
+    if (c <= 128) return launch_rows<T, 64, 2>(a, threads, stream);
+    if (c <= 256) return launch_rows<T, 64, 4>(a, threads, stream);
+    if (c <= 512) return launch_rows<T, 256, 2>(a, threads, stream);
+    if (c <= 2048 && a.M <= 256) return launch_rows<T, 1024, 2>(a, threads, stream);
+    if (c <= 1024) return launch_rows<T, 256, 4>(a, threads, stream);
+    if (c <= 2048) return launch_rows<T, 256, 8>(a, threads, stream);
+    if (c <= 4096) return launch_rows<T, 1024, 4>(a, threads, stream);
+    return launch_row_ranges(a, threads, sizeof(T), 1024, 1, [&](const QuantRowsArgs& part, dim3 grid) {
         return enqueue(a.norm ? quant_long_rows_kernel<T, true> : quant_long_rows_kernel<T, false>, grid, 1024, 0, stream, part);
     });
 }
 
-D4PG_API int d4pg_quant_rows(const QuantRowsArgs* a, hipStream_t stream) {
+D4PG_API int d4pg_quant_rows_in(const QuantRowsArgs* a, long long threads, hipStream_t stream) {
+    if (!good_limit(threads)) return -8;
     if (a->M < 1 || a->M > 0x7fffffffll || a->K < 1 || a->K > 0x7fffffffll) return -1;
     if (a->x == nullptr || a->q == nullptr || a->scale == nullptr) return -2;
     if ((a->ld_q & 15) || a->ld_q < a->K || a->ld_q >= a->K + 16 || ((uintptr_t)a->q & 15)) return -3;
     if (a->wdtype != F_NONE && (a->weight == nullptr || a->wdtype < 0 || a->wdtype > F_FP16)) return -4;
     if (!a->norm && (a->residual != nullptr || a->weight != nullptr || a->h != nullptr)) return -5;
-    if (a->dtype == F_FP32) return launch_rows_of<float>(*a, stream);
-    if (a->dtype == F_BF16) return launch_rows_of<__bf16>(*a, stream);
-    if (a->dtype == F_FP16) return launch_rows_of<_Float16>(*a, stream);
+    if (a->dtype == F_FP32) return launch_rows_of<float>(*a, threads, stream);
+    if (a->dtype == F_BF16) return launch_rows_of<__bf16>(*a, threads, stream);
+    if (a->dtype == F_FP16) return launch_rows_of<_Float16>(*a, threads, stream);
     return -6;
 }
+D4PG_API int d4pg_quant_rows(const QuantRowsArgs* a, hipStream_t stream) { return d4pg_quant_rows_in(a, LAUNCH_THREADS, stream); }
 
 // ---------------------------------------------------------------------------------------------------------------
 // codes -> floating rows
@@ -485,16 +492,17 @@ __global__ __launch_bounds__(256) void dequant_rows_kernel(const DequantRowsArgs
     }
 }
 
-D4PG_API int d4pg_dequant_rows(DequantRowsArgs* a, hipStream_t stream) {
+D4PG_API int d4pg_dequant_rows_in(DequantRowsArgs* a, long long threads, hipStream_t stream) {
+    if (!good_limit(threads)) return -8;
     if (a->M < 1 || a->M > 0x7fffffffll || a->K < 1 || a->K > 0x7fffffffll) return -1;
     if (a->q == nullptr || a->scale == nullptr || a->out == nullptr) return -2;
     a->tpr_log = 0;
     while (a->tpr_log < 8 && (8ll << a->tpr_log) < a->K) ++a->tpr_log;
     const int rpb = 256 >> a->tpr_log;
-    const long long most = (0xffffffffll / 256) * rpb;
+    const long long most = (threads / 256) * rpb;
     const int bytes = a->dtype == F_FP32 ? 4 : 2;
     if (a->dtype < F_FP32 || a->dtype > F_FP16) return -6;
-    for (long long done = 0; done < a->M; done += most) {       // fewer than 2^32 threads a launch
+    for (long long done = 0; done < a->M; done += most) {
         DequantRowsArgs part = *a;
         part.M = a->M - done < most ? a->M - done : most;
         part.q = a->q + done * a->ld_q, part.scale = a->scale + done, part.out = (char*)a->out + done * a->K * bytes;
@@ -507,6 +515,7 @@ D4PG_API int d4pg_dequant_rows(DequantRowsArgs* a, hipStream_t stream) {
     }
     return 0;
 }
+D4PG_API int d4pg_dequant_rows(DequantRowsArgs* a, hipStream_t stream) { return d4pg_dequant_rows_in(a, LAUNCH_THREADS, stream); }
 
 // ---------------------------------------------------------------------------------------------------------------
 // product of codes
@@ -591,7 +600,7 @@ __device__ __forceinline__ void finish4(const LinearInt8Args& a, int m, int n, c
     store_values4(a.out, (long long)m * a.ld_out + n, a.dtype, v, a.N - n);
 }
 
-enum { TOO_MANY = -7 };        // threads for one launch: the caller halves the rows
+enum { TOO_MANY = -7 };        // threads for one launch: the caller halves the rows (16 rows fit the real limit whatever their columns)
 
 // All ones in the bytes k .. k + 15 that lie below K.
 __device__ __forceinline__ i32x4 below(int k, int K) {
@@ -677,9 +686,9 @@ __global__ __launch_bounds__(64 * WAVES) void linear_int8_rows_kernel(const Line
 }
 
 template <int MT, int NT, int WAVES, int U>
-static int launch_linear_rows(const LinearInt8Args& a, hipStream_t stream) {
+static int launch_linear_rows(const LinearInt8Args& a, long long threads, hipStream_t stream) {
     const long long tiles = (long long)((a.M + 16 * MT - 1) / (16 * MT)) * ((a.N + 16 * NT - 1) / (16 * NT));
-    if (tiles * (64 * WAVES) > 0xffffffffll) return TOO_MANY;
+    if (tiles * (64 * WAVES) > threads) return TOO_MANY;
     return enqueue(linear_int8_rows_kernel<MT, NT, WAVES, U>, dim3((unsigned)tiles), 64 * WAVES, 0, stream, a);
 }
 
@@ -838,11 +847,11 @@ __global__ __launch_bounds__(64 * WM * WN * KW, WM * WN * KW / 4 * (MI * NI * WM
 }
 
 template <int MI, int NI, int WM, int WN, int KW, int S>
-static int launch_linear_tiles(const LinearInt8Args& a, hipStream_t stream) {
+static int launch_linear_tiles(const LinearInt8Args& a, long long threads, hipStream_t stream) {
     constexpr int BM = 32 * MI * WM, BN = 32 * NI * WN, TILES = S * (BM + BN) * 128, STAGE = WM * WN * (32 * (32 * NI + 4) * 4 + (KW == 2 ? NI * MI * 4096 : 0));
     constexpr int LDS = TILES > STAGE ? TILES : STAGE;
     const long long tiles = (long long)((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN);
-    if (tiles * (64 * WM * WN * KW) > 0xffffffffll) return TOO_MANY;
+    if (tiles * (64 * WM * WN * KW) > threads) return TOO_MANY;
     return enqueue(linear_int8_tiles_kernel<MI, NI, WM, WN, KW, S>, dim3((unsigned)tiles), 64 * WM * WN * KW, LDS, stream, a);
 }
 
@@ -873,47 +882,48 @@ static int launch_linear_tiles(const LinearInt8Args& a, hipStream_t stream) {
 // workgroups (one set of operands, 256 x 400 x 400: 3.7 with 2 x 1 tiles, 4.0 with 1 x 1, 4.2 with 2 x 2; 512 x 1024 x 1024: 6.3 with 4 x 2, 6.9
 // with 2 x 2, 8.6 with 2 x 1; 1 x 16384 x 4096: 12.8 with 1 x 4, 14.6 with 1 x 1), and K is dealt to 16 waves where it is long
 // and the workgroups are few (1 x 4096 x 4096: 5.5 with 16 waves, 6.5 with 4; 1 x 1333 x 2001: 4.4 and 3.6).
-static int launch_linear(const LinearInt8Args& a, long long kp, hipStream_t stream) {
+static int launch_linear(const LinearInt8Args& a, long long kp, long long threads, hipStream_t stream) {
     auto tiles = [&](int side) { return (long long)((a.M + side - 1) / side) * ((a.N + side - 1) / side); };
     // the tile kernel's offsets inside 256 rows are 32-bit
     if (256 * (a.M > 1 ? a.ld_q : kp) + kp < 0x7fffffffll && 256 * (a.N > 1 ? a.ld_w : kp) + kp < 0x7fffffffll) {
-        if (a.M > 128 && tiles(256) >= 192) return launch_linear_tiles<2, 2, 4, 4, 1, 2>(a, stream);
-        if (a.M > 64 && tiles(128) > 256) return launch_linear_tiles<2, 1, 2, 4, 1, 2>(a, stream);
-        if (a.M > 64 && tiles(128) >= 144 && a.K >= 2048) return launch_linear_tiles<1, 1, 4, 4, 1, 4>(a, stream);
+        if (a.M > 128 && tiles(256) >= 192) return launch_linear_tiles<2, 2, 4, 4, 1, 2>(a, threads, stream);
+        if (a.M > 64 && tiles(128) > 256) return launch_linear_tiles<2, 1, 2, 4, 1, 2>(a, threads, stream);
+        if (a.M > 64 && tiles(128) >= 144 && a.K >= 2048) return launch_linear_tiles<1, 1, 4, 4, 1, 4>(a, threads, stream);
         if ((a.M > 32 && tiles(64) >= 128) || (a.M > 16 && tiles(64) >= 256 && a.K >= 2048)) {
-            if (a.K >= 4096 || (a.K >= 1024 && tiles(64) <= 384)) return launch_linear_tiles<1, 1, 2, 2, 2, 4>(a, stream);
-            return launch_linear_tiles<1, 1, 2, 2, 1, 2>(a, stream);
+            if (a.K >= 4096 || (a.K >= 1024 && tiles(64) <= 384)) return launch_linear_tiles<1, 1, 2, 2, 2, 4>(a, threads, stream);
+            return launch_linear_tiles<1, 1, 2, 2, 1, 2>(a, threads, stream);
         }
     }
     const long long t = tiles(16);
     if (a.M <= 16) {
-        if (t >= 768) return launch_linear_rows<1, 4, 4, 1>(a, stream);
-        if (t <= 256 && a.K >= 4096) return launch_linear_rows<1, 1, 16, 4>(a, stream);
-        return launch_linear_rows<1, 1, 4, 2>(a, stream);
+        if (t >= 768) return launch_linear_rows<1, 4, 4, 1>(a, threads, stream);
+        if (t <= 256 && a.K >= 4096) return launch_linear_rows<1, 1, 16, 4>(a, threads, stream);
+        return launch_linear_rows<1, 1, 4, 2>(a, threads, stream);
     }
-    if (t <= 320) return launch_linear_rows<1, 1, 4, 2>(a, stream);
-    if (t <= 640) return launch_linear_rows<2, 1, 8, 2>(a, stream);
-    if (t <= 1536) return launch_linear_rows<2, 2, 4, 4>(a, stream);
-    if (a.M <= 32) return launch_linear_rows<2, 4, 4, 2>(a, stream);
-    return launch_linear_rows<4, 2, 8, 2>(a, stream);
+    if (t <= 320) return launch_linear_rows<1, 1, 4, 2>(a, threads, stream);
+    if (t <= 640) return launch_linear_rows<2, 1, 8, 2>(a, threads, stream);
+    if (t <= 1536) return launch_linear_rows<2, 2, 4, 4>(a, threads, stream);
+    if (a.M <= 32) return launch_linear_rows<2, 4, 4, 2>(a, threads, stream);
+    return launch_linear_rows<4, 2, 8, 2>(a, threads, stream);
 }
 
-static int linear_rows_of(const LinearInt8Args& a, long long kp, hipStream_t stream) {
-    int rc = a.M > 1 << 30 ? (int)TOO_MANY : launch_linear(a, kp, stream);      // row numbers past M stay 32-bit
+static int linear_rows_of(const LinearInt8Args& a, long long kp, long long threads, hipStream_t stream) {
+    int rc = a.M > 1 << 30 ? (int)TOO_MANY : launch_linear(a, kp, threads, stream);      // row numbers past M stay 32-bit
     if (rc != TOO_MANY || a.M <= 16) return rc;
     const int whole = a.M > 512 ? 255 : 15;
     const long long done = (a.M / 2 + whole) & ~whole;
     LinearInt8Args part = a;
     part.M = (int)done;
-    rc = linear_rows_of(part, kp, stream);
+    rc = linear_rows_of(part, kp, threads, stream);
     if (rc != 0) return rc;
     part = a;
     part.M -= (int)done, part.q += done * a.ld_q, part.scale += done;
     part.out = (char*)a.out + done * a.ld_out * (a.dtype == F_FP32 ? 4 : 2);
-    return linear_rows_of(part, kp, stream);
+    return linear_rows_of(part, kp, threads, stream);
 }
 
-D4PG_API int d4pg_linear_int8(const LinearInt8Args* a, hipStream_t stream) {
+D4PG_API int d4pg_linear_int8_in(const LinearInt8Args* a, long long threads, hipStream_t stream) {
+    if (!good_limit(threads)) return -8;
     if (a->M < 1 || a->N < 1 || a->N > 1 << 29 || a->K < 1 || a->K >= 131072) return -1;
     if (a->q == nullptr || a->w == nullptr || a->scale == nullptr || a->wscale == nullptr || a->out == nullptr) return -2;
     const long long kp = (a->K + 15) & ~15;
@@ -921,8 +931,9 @@ D4PG_API int d4pg_linear_int8(const LinearInt8Args* a, hipStream_t stream) {
     if ((a->M > 1 && a->ld_q < kp) || (a->N > 1 && a->ld_w < kp) || (a->M > 1 && a->ld_out < a->N)) return -4;
     if (((uintptr_t)a->q | (uintptr_t)a->w) & 15) return -5;
     if (a->dtype < F_FP32 || a->dtype > F_FP16 || a->act < ACT_NONE || a->act > ACT_TANH) return -6;
-    return linear_rows_of(*a, kp, stream);
+    return linear_rows_of(*a, kp, threads, stream);
 }
+D4PG_API int d4pg_linear_int8(const LinearInt8Args* a, hipStream_t stream) { return d4pg_linear_int8_in(a, LAUNCH_THREADS, stream); }
 
 // ---------------------------------------------------------------------------------------------------------------
 // three layers on codes in one launch

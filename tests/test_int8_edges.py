@@ -261,3 +261,98 @@ def test_a_launch_that_hip_refuses_raises_and_is_not_tried_again():
     finally:
         binding.bind(*real)
     assert torch.equal(ops.quantize_rows(x)[0], q)
+
+
+# ------------------------------------------------------------------------------------- more rows than one launch may hold
+def _launches(call):
+    """Kernel launches of ``call`` (0 is what it returns), which then run once."""
+    from d4pg_pytorch_amd.ops import hip as H
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        rc = call(torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    n = H.graph_kernel_nodes(graph)
+    graph.instantiate()
+    graph.replay()
+    torch.cuda.synchronize()
+    return n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K", [(1000, 40), (1000, 128), (999, 250), (1000, 500), (300, 1000), (300, 2000), (90, 4000), (30, 5001),
+                                 (300, 5001), (300, 9001), (30, 20000), (9, 40001)])
+def test_rows_of_several_launches(M, K):
+    """Every row kernel with a limit of 4096 threads a launch: the same bits as in one launch, the rows' ends included."""
+    import ctypes as C
+
+    from d4pg_pytorch_amd.ops import hip as H
+    kp = (K + 15) // 16 * 16
+    for dtype, code in ((torch.bfloat16, H.F_BF16), (torch.float32, H.F_FP32)):
+        x, r, g = (_randn(*shape, seed=i).to(dtype).cuda() for i, shape in enumerate(((M, K + 3), (M, K), (K,))))
+        x = x[:, 2:2 + K]
+        for norm in (0, 1):
+            want = ops.add_rms_norm_int8(x, g, r) if norm else ops.quantize_rows(x)
+            q, s, h = torch.full((M, kp), 99, dtype=torch.int8, device="cuda"), torch.full((M,), -1.0, device="cuda"), torch.zeros_like(r)
+            a = H.QuantRowsArgs(x.data_ptr(), None, None, None, q.data_ptr(), s.data_ptr(), M, K, K + 3, 0, 0, kp, code, H.F_NONE, 0, 0.0)
+            if norm:
+                a.residual, a.weight, a.h, a.ld_r, a.ld_h = r.data_ptr(), g.data_ptr(), h.data_ptr(), K, K
+                a.wdtype, a.norm, a.eps = code, 1, 1e-6
+            assert _launches(lambda stream: H.lib().d4pg_quant_rows_in(C.byref(a), 4096, stream)) > 1
+            assert torch.equal(q[:, :K], want[0]) and not q[:, K:].any() and torch.equal(s, want[1])
+            assert not norm or torch.equal(h, want[2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K", [(3000, 1), (2999, 9), (777, 100), (20, 5001)])
+def test_values_of_several_launches(M, K):
+    import ctypes as C
+
+    from d4pg_pytorch_amd.ops import hip as H
+    q, s = ops.quantize_rows(_randn(M, K, seed=K).cuda())
+    for dtype, code in ((torch.float32, H.F_FP32), (torch.float16, H.F_FP16)):
+        out = torch.full((M, K), 7.0, dtype=dtype, device="cuda")
+        a = H.DequantRowsArgs(q.data_ptr(), s.data_ptr(), out.data_ptr(), M, K, q.stride(0), code, 0)
+        assert _launches(lambda stream: H.lib().d4pg_dequant_rows_in(C.byref(a), 1024, stream)) > 1
+        assert torch.equal(out, ops.dequantize_rows(q, s, dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K,threads", [(500, 950, 333, 16384), (777, 130, 2001, 3000), (2300, 1700, 130, 40000), (513, 1, 1, 1024),
+                                           (1000, 70, 4100, 60000), (33, 3000, 50, 50000)])
+def test_products_of_several_launches(M, N, K, threads):
+    import ctypes as C
+
+    from d4pg_pytorch_amd.ops import hip as H
+    q, s = ops.quantize_rows(_randn(M, K, seed=1).cuda())
+    w, ws = ops.quantize_rows(_randn(N, K, seed=2).cuda())
+    b = _randn(N, seed=3).cuda()
+    for dtype, code in ((torch.float32, H.F_FP32), (torch.bfloat16, H.F_BF16)):
+        out = torch.full((M + 1, N), 7.0, dtype=dtype, device="cuda")
+        a = H.LinearInt8Args(q.data_ptr(), s.data_ptr(), w.data_ptr(), ws.data_ptr(), b.data_ptr(), out.data_ptr(), q.stride(0), w.stride(0), N,
+                             M, N, K, H.ACT_RELU, code, 0)
+        assert _launches(lambda stream: H.lib().d4pg_linear_int8_in(C.byref(a), threads, stream)) > 1
+        assert torch.equal(out[:M], ops.linear_int8(q, s, w, ws, b, "relu", dtype)) and torch.all(out[M] == 7)
+
+
+@pytest.mark.gpu
+def test_more_rows_than_the_real_limit():
+    """16 threads a row: 2^28 rows of one column are 2^32 threads.  The rows are one in memory, so that codes, scales and
+    what checks them are all there is (4 GB of codes, one of scales)."""
+    M = (1 << 28) + 70
+    x = torch.full((1, 1), -3.0, device="cuda").expand(M, 1)
+    q, s = ops.quantize_rows(x)
+    want = torch.tensor(3.0) / 127
+    for part in range(0, M, 1 << 26):
+        assert torch.all(q[part:part + (1 << 26)] == -127) and torch.all(s[part:part + (1 << 26)] == want.item())
+
+
+def test_limits_a_launch_cannot_have_are_refused():
+    import ctypes as C
+
+    from d4pg_pytorch_amd.ops import hip as H
+    lib = H.lib()
+    for limit in (0, 1023, -1, 1 << 32):
+        assert lib.d4pg_quant_rows_in(C.byref(H.QuantRowsArgs()), limit, None) == -8
+        assert lib.d4pg_dequant_rows_in(C.byref(H.DequantRowsArgs()), limit, None) == -8
+        assert lib.d4pg_linear_int8_in(C.byref(H.LinearInt8Args()), limit, None) == -8
+    assert lib.d4pg_linear_int8_in(C.byref(H.LinearInt8Args()), 1024, None) == -1
