@@ -356,3 +356,76 @@ def test_limits_a_launch_cannot_have_are_refused():
         assert lib.d4pg_dequant_rows_in(C.byref(H.DequantRowsArgs()), limit, None) == -8
         assert lib.d4pg_linear_int8_in(C.byref(H.LinearInt8Args()), limit, None) == -8
     assert lib.d4pg_linear_int8_in(C.byref(H.LinearInt8Args()), 1024, None) == -1
+
+
+# --------------------------------------------------------------------- kernels of the dispatch that no other test reaches
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,dims", [(4097, (24, 400, 400, 4)), (4131, (17, 256, 250, 129)), (4100, (100, 130, 77, 256)), (4127, (33, 60, 512, 9)),
+                                    (4112, (200, 500, 300, 500)), (4133, (111, 1024, 1024, 8)), (4099, (64, 1000, 90, 1024)), (8209, (5, 128, 1024, 1)),
+                                    (4105, (3, 16, 128, 65)), (4098, (700, 1024, 1024, 1024))])
+def test_mlp3_int8_by_32_rows_a_workgroup(B, dims):
+    """More than 4096 states: the kernels that take 32 rows at a time, with ragged ends, wide and narrow layers in every
+    place, and rows that are not finite in both halves of 16; to the last bit as the layers one by one."""
+    x = _randn(B, dims[0], seed=B).cuda()
+    x[20, dims[0] // 2], x[5, 0], x[B - 1, 0], x[17] = math.nan, math.inf, -math.inf, 0.0
+    layers = []
+    for i in range(3):
+        bias = 0.1 * _randn(dims[i + 1], seed=i).cuda() if (B + i) % 2 else None
+        layers.append((*ops.quantize_rows((_randn(dims[i + 1], dims[i], seed=B + i) / math.sqrt(dims[i])).cuda()), bias))
+    for final, dtype, xt in (("tanh", torch.float32, torch.float32), ("none", torch.bfloat16, torch.bfloat16), ("relu", torch.float16, torch.float16)):
+        want = x.to(xt)
+        for i, (w, ws, b) in enumerate(layers):
+            want = ops.linear_int8(*ops.quantize_rows(want), w, ws, b, "relu" if i < 2 else final, torch.float32 if i < 2 else dtype)
+        got = ops.mlp3_int8(x.to(xt), layers, final, dtype)
+        assert torch.isnan(got[[5, 20, B - 1]]).all() and torch.equal(torch.isnan(got), torch.isnan(want))
+        assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(500, 950, 333), (1900, 250, 1111), (127, 4000, 40), (1500, 200, 1000), (33, 16000, 30)])
+def test_linear_int8_between_the_row_kernels_and_the_tiles(M, N, K):
+    """Fewer than 128 tiles of 64 x 64, more than 1536 of 16 x 16 (``linear_int8_rows_kernel<4, 2, 8, 2>``), and around it."""
+    from test_int8 import _linear_case
+    _linear_case(M, N, K, "cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,K", [(300, 5003), (300, 8200), (257, 9001), (1000, 4104), (256, 5003), (256, 16384), (257, 16384)])
+def test_quantize_long_rows_of_many(M, K, dtype):
+    x = (_randn(M, K, seed=M + K) * torch.exp(2 * _randn(M, 1, seed=5))).to(dtype).cuda()
+    x[3, K - 1], x[4] = math.nan, 0.0
+    q, scale = ops.quantize_rows(x)
+    assert torch.isnan(scale[3]) and not q[3].any() and scale[4] == 0 and not q[4].any()
+    rows = [i for i in range(M) if i not in (3, 4)]
+    _check_codes(q[rows], scale[rows], x[rows], 0.0)
+
+
+@pytest.mark.gpu
+def test_threads_on_streams_of_their_own_all_come_to_their_end():
+    """Four threads, each on its own stream: what goes wrong in one is seen, and each has made all of its calls."""
+    import threading
+    layers = [(*ops.quantize_rows((_randn(n, k, seed=n + k) / math.sqrt(k)).cuda()), None) for n, k in ((256, 100), (256, 256), (5, 256))]
+    xs = [_randn(300, 100, seed=i).cuda() for i in range(4)]
+    want = [(*ops.add_rms_norm_int8(x, None, x), ops.mlp3_int8(x, layers, "tanh"), ops.linear_int8(*ops.quantize_rows(x), *layers[0])) for x in xs]
+    torch.cuda.synchronize()
+    done, wrong = [0] * 4, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(50):
+                    x = xs[i]
+                    got = (*ops.add_rms_norm_int8(x, None, x), ops.mlp3_int8(x, layers, "tanh"), ops.linear_int8(*ops.quantize_rows(x), *layers[0]))
+                    if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                        wrong.append(f"thread {i}: other values")
+                    done[i] += 1
+        except BaseException as e:                      # noqa: BLE001
+            wrong.append(f"thread {i}: {e!r}")
+
+    threads = [threading.Thread(target=work, args=(i,), daemon=True) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not wrong and done == [50] * 4 and not any(t.is_alive() for t in threads)
