@@ -1266,7 +1266,7 @@ D4PG_API int d4pg_mlp3_int8(Mlp3Int8Args* a, hipStream_t stream) {
     if (a->act < ACT_NONE || a->act > ACT_TANH) return -6;
     int widest = 0, wide_out = 0, few = 0;
     for (int i = 0; i < 4; ++i) {
-        if (a->width[i] < 1) return -1;
+        if (a->width[i] < 1 || a->width[i] > 1 << 29) return -1;       // as in the product; rounded up to tiles they stay 32-bit
         if (i < 3 && a->width[i] > widest) widest = a->width[i];
     }
     for (int i = 0; i < 3; ++i) {

@@ -202,6 +202,17 @@ def test_a_policy_outside_the_one_launch_is_told_from_an_error():
         assert H.lib().d4pg_mlp3_int8(C.byref(a), None) == H.NOT_TAKEN < 0, dims
 
 
+def test_a_policy_of_too_many_columns_is_refused():
+    """Numbers of columns that leave 32 bits when they are rounded up to tiles; nothing is launched."""
+    import ctypes as C
+
+    from d4pg_pytorch_amd.ops import hip as H
+    a, *held = _policy(3, [16, 64, 64, 4], "cpu")
+    for width in ((1 << 31) - 1, (1 << 31) - 20, (1 << 29) + 1):
+        a.width[3] = a.ld_out = width
+        assert H.lib().d4pg_mlp3_int8(C.byref(a), None) == -1
+
+
 @pytest.mark.gpu
 def test_an_error_left_by_another_call_is_not_taken_for_an_operators_own():
     import ctypes as C
