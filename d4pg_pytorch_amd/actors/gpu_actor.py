@@ -19,7 +19,7 @@ Hidden widths outside the fused kernel's set fall back to three launches of the 
 GEMM (``csrc/gemm.hip``).
 
 ``precision="int8"`` answers with 8-bit codes instead: the weights are quantised per output channel whenever new
-parameters arrive, states and hidden activations per row (``ops/int8.py::mlp3_int8``, one launch up to 1024 columns).
+parameters arrive, states and hidden activations per row (``ops/int8.py::mlp3_int8``).
 """
 from __future__ import annotations
 
@@ -158,8 +158,8 @@ class GpuActor:
         elif self.fused is None:         # per-layer path: two hidden activation buffers
             self.h1 = torch.zeros(self.E, ldh, device=self.device)
             self.h2 = torch.zeros(self.E, ldh, device=self.device)
-        if precision == "int8":        # the network (a launch a step beyond 1024 columns) and the way into the caller's actions
-            self.launches_per_act = 2 if max(state_dim, hidden) <= 1024 else 7
+        if precision == "int8":        # the network for ``max_batch`` states, and the way into the caller's actions
+            self.launches_per_act = H.lib().d4pg_mlp3_int8_launches(self.E, state_dim, hidden, hidden, action_dim) + 1
         else:
             self.launches_per_act = 1 if self.fused is not None else 3
         self._shared = None

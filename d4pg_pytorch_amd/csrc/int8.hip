@@ -1250,41 +1250,63 @@ __global__ __launch_bounds__(64 * MLP_WAVES) void mlp3_int8_kernel(const Mlp3Int
     mlp3_rows<TPW, MT>(a, net);
 }
 
-// NOT_TAKEN: does not fit the LDS
+// How the one launch takes a network, from its widths and rows alone.
+struct MlpPlan {
+    int tpw, mt;                   // tiles of 16 columns a wave, 16-row tiles a workgroup
+    int pitch, split, lds;
+};
+// 0, NOT_TAKEN or a refusal
+static int mlp_plan(int M, const int (&width)[4], MlpPlan& p) {
+    if (M < 1) return -1;
+    int widest = 0, wide_out = 0, few = 0;
+    for (int i = 0; i < 4; ++i) {
+        if (width[i] < 1 || width[i] > 1 << 29) return -1;         // as in the product; rounded up to tiles they stay 32-bit
+        if (i < 3 && width[i] > widest) widest = width[i];
+        const int tiles = (width[i] + 15) / 16;
+        if (i > 0 && tiles > wide_out) wide_out = tiles;
+        if (i > 0 && tiles <= MLP_WAVES / 2 && tiles > few) few = tiles;
+    }
+    if (widest > 2048 || wide_out > 64 || M > 1 << 25) return NOT_TAKEN;       // (2^25 rows: 2^31 threads)
+    p.tpw = wide_out <= 16 ? 1 : wide_out <= 32 ? 2 : 4;
+    p.mt = M > 4096 ? 2 : 1;       // 32 rows a workgroup, so that one round of workgroups holds them longer
+    p.pitch = ((widest + 63) & ~63) + 16;
+    p.split = few * p.mt * 256;
+    p.lds = MLP_WAVES * (mlp_ring(p.mt) * 1024 + 512) + 16 * p.mt * p.pitch + 4 * p.split + 3 * 16 * p.mt * 4;
+    return p.lds > 160 * 1024 ? (int)NOT_TAKEN : 0;
+}
+
 template <int TPW, int MT>
-static int launch_mlp3(Mlp3Int8Args& a, int few, hipStream_t stream) {
-    a.split = few * MT * 256;
-    const int lds = MLP_WAVES * (mlp_ring(MT) * 1024 + 512) + 16 * MT * a.pitch + 4 * a.split + 3 * 16 * MT * 4;
-    if (lds > 160 * 1024) return NOT_TAKEN;
+static int launch_mlp3(const Mlp3Int8Args& a, int lds, hipStream_t stream) {
     return enqueue(mlp3_int8_kernel<TPW, MT>, dim3((unsigned)((a.M + 16 * MT - 1) / (16 * MT))), 64 * MLP_WAVES, lds, stream, a);
 }
 
 // NOT_TAKEN: outside this kernel's range.
 D4PG_API int d4pg_mlp3_int8(Mlp3Int8Args* a, hipStream_t stream) {
-    if (a->M < 1 || a->x == nullptr || a->out == nullptr || a->ld_out < a->width[3]) return -1;
+    if (a->x == nullptr || a->out == nullptr || a->ld_out < a->width[3]) return -1;
     if (a->dtype < F_FP32 || a->dtype > F_FP16 || a->xdtype < F_FP32 || a->xdtype > F_FP16) return -6;
     if (a->act < ACT_NONE || a->act > ACT_TANH) return -6;
-    int widest = 0, wide_out = 0, few = 0;
-    for (int i = 0; i < 4; ++i) {
-        if (a->width[i] < 1 || a->width[i] > 1 << 29) return -1;       // as in the product; rounded up to tiles they stay 32-bit
-        if (i < 3 && a->width[i] > widest) widest = a->width[i];
-    }
+    MlpPlan p;
+    const int rc = mlp_plan(a->M, a->width, p);
+    if (rc != 0 && rc != NOT_TAKEN) return rc;
     for (int i = 0; i < 3; ++i) {
         const long long kp = (a->width[i] + 15) & ~15;
         if (a->w[i] == nullptr || a->wscale[i] == nullptr) return -2;
         if (((uintptr_t)a->w[i] & 15) || (a->width[i + 1] > 1 && ((a->ld_w[i] & 15) || a->ld_w[i] < kp))) return -3;
         if (a->ld_w[i] >= 1 << 20) return NOT_TAKEN;        // offsets inside a matrix are 32-bit
-        const int tiles = (a->width[i + 1] + 15) / 16;
-        if (tiles > wide_out) wide_out = tiles;
-        if (tiles <= MLP_WAVES / 2 && tiles > few) few = tiles;
     }
-    if (widest > 2048 || wide_out > 64 || a->M > 1 << 25) return NOT_TAKEN;       // (2^25 rows: 2^31 threads)
-    a->pitch = ((widest + 63) & ~63) + 16;
-    const bool two = a->M > 4096;                // 32 rows a workgroup, so that one round of workgroups holds them longer
-    if (wide_out <= 16) return two ? launch_mlp3<1, 2>(*a, few, stream) : launch_mlp3<1, 1>(*a, few, stream);
-    if (wide_out <= 32) return two ? launch_mlp3<2, 2>(*a, few, stream) : launch_mlp3<2, 1>(*a, few, stream);
-    if (two) return launch_mlp3<4, 2>(*a, few, stream);
-    return launch_mlp3<4, 1>(*a, few, stream);
+    if (rc != 0) return rc;
+    a->pitch = p.pitch, a->split = p.split;
+    if (p.tpw == 1) return p.mt == 2 ? launch_mlp3<1, 2>(*a, p.lds, stream) : launch_mlp3<1, 1>(*a, p.lds, stream);
+    if (p.tpw == 2) return p.mt == 2 ? launch_mlp3<2, 2>(*a, p.lds, stream) : launch_mlp3<2, 1>(*a, p.lds, stream);
+    return p.mt == 2 ? launch_mlp3<4, 2>(*a, p.lds, stream) : launch_mlp3<4, 1>(*a, p.lds, stream);
+}
+
+// Launches that M rows through a network of these widths (densely stored weights) take: 1, or 6, a quantisation and a product
+// a layer; < 0: refused.
+D4PG_API int d4pg_mlp3_int8_launches(int M, int w0, int w1, int w2, int w3) {
+    MlpPlan p;
+    const int rc = mlp_plan(M, {w0, w1, w2, w3}, p);
+    return rc == 0 ? 1 : rc == NOT_TAKEN ? 6 : rc;
 }
 
 D4PG_SIZEOF(Mlp3Int8Args)

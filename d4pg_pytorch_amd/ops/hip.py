@@ -504,6 +504,7 @@ def lib() -> C.CDLL:
             ("d4pg_quant_rows_in", [C.POINTER(QuantRowsArgs), C.c_longlong, vp]),
             ("d4pg_dequant_rows_in", [C.POINTER(DequantRowsArgs), C.c_longlong, vp]),
             ("d4pg_linear_int8_in", [C.POINTER(LinearInt8Args), C.c_longlong, vp]),
+            ("d4pg_mlp3_int8_launches", [C.c_int] * 5),
             ("d4pg_mlp3_int8", [C.POINTER(Mlp3Int8Args), vp]),
             ("d4pg_ipc_alloc", [C.c_size_t, C.POINTER(vp), C.c_char_p]),
             ("d4pg_ipc_open", [C.c_char_p, C.POINTER(vp)]),

@@ -294,7 +294,9 @@ def mlp3_int8(x: torch.Tensor, layers: Sequence[Tuple[torch.Tensor, torch.Tensor
 
     ``x[..., S]`` fp32, bf16 or fp16; ``layers``: three ``(weight[out, in] int8, weight_scale[out], bias[out] or None)``.
     The input of every layer is quantised per row; what the layers hand on is fp32; the result is in ``dtype``.  On the GPU
-    the network is one launch (``mlp3_int8_kernel``) up to 1024 columns, and a launch per step beyond what its LDS holds."""
+    the network is one launch (``mlp3_int8_kernel``) where no layer has more than 1024 outputs and the LDS holds it: always up
+    to 1024 columns, except for a layer of 113 - 128 outputs beside one of more than 960 inputs with up to 4096 states.
+    Otherwise it is a quantisation and a product a layer (``d4pg_mlp3_int8_launches`` says which)."""
     if x.is_cuda and len(layers) == 3:
         out = _binding().mlp3(x, *layers[0], *layers[1], *layers[2], _ACTS.get(final, -1), _FLOATS.get(dtype, -1))
         if out is not None:

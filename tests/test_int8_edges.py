@@ -440,3 +440,34 @@ def test_threads_on_streams_of_their_own_all_come_to_their_end():
     for t in threads:
         t.join(60)
     assert not wrong and done == [50] * 4 and not any(t.is_alive() for t in threads)
+
+
+# ------------------------------------------------------------------------------------------------ launches, as they are told
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,dims", [(1, (24, 400, 400, 4)), (3, (111, 1024, 1024, 8)), (3, (64, 1024, 1024, 120)), (4097, (64, 1024, 1024, 120)),
+                                    (2, (961, 16, 16, 128)), (2, (960, 16, 16, 128)), (2, (2048, 64, 64, 2)), (2, (3, 1025, 64, 2)), (5, (8, 64, 64, 1025))])
+def test_the_policys_launches_are_told_as_they_are(M, dims):
+    from d4pg_pytorch_amd.ops import hip as H
+    x = _randn(M, dims[0], seed=1).cuda()
+    layers = [(*ops.quantize_rows(_randn(dims[i + 1], dims[i], seed=i).cuda()), None) for i in range(3)]
+    ops.mlp3_int8(x, layers)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        ops.mlp3_int8(x, layers)
+    assert H.graph_kernel_nodes(graph) == H.lib().d4pg_mlp3_int8_launches(M, *dims)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S,Hd,A,E", [(24, 400, 4, 16), (64, 1024, 120, 8), (64, 1024, 120, 4097), (3, 1100, 1, 2)])
+def test_an_agent_tells_its_launches_as_they_are(S, Hd, A, E):
+    from d4pg_pytorch_amd.actors.gpu_actor import GpuActor
+    from d4pg_pytorch_amd.ops import hip as H
+    ga = GpuActor(S, A, Hd, max_batch=E, precision="int8")
+    obs = _randn(E, S, seed=1).cuda()
+    ga.act_device(obs)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        ga.act_device(obs)
+    assert H.graph_kernel_nodes(graph) == ga.launches_per_act
