@@ -8,7 +8,8 @@ Activations are quantised per row (token, state), weights per output channel (th
     y = linear_int8(q, s, wq, ws, layer.bias, "relu", torch.bfloat16)
 
 On a ROCm tensor the functions launch the kernels of ``csrc/int8.hip`` on the current stream of the tensors' device; on a
-CPU tensor they evaluate ``ops/ref.py``.  They serve: no gradient flows through codes, and what they return requires none.
+CPU tensor they evaluate ``ops/ref.py``.  They serve: no gradient flows through codes, and what they make requires none
+(``add_rms_norm_int8`` without a residual hands back ``x`` itself as ``h``, which requires what ``x`` requires).
 
 Code matrices are handed out with rows padded to 16 bytes (a view of ``[..., K]`` codes whose row stride is the next
 multiple of 16), which is what the product reads directly; codes laid out differently are copied once per call.

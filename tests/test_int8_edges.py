@@ -471,3 +471,46 @@ def test_an_agent_tells_its_launches_as_they_are(S, Hd, A, E):
     with torch.cuda.graph(graph):
         ga.act_device(obs)
     assert H.graph_kernel_nodes(graph) == ga.launches_per_act
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_what_requires_gradients_afterwards(device):
+    x = _randn(3, 20, seed=1).to(device).requires_grad_()
+    q, s, h = ops.add_rms_norm_int8(x, x.detach()[0].clone().requires_grad_(), x)
+    assert not any(t.requires_grad for t in (q, s, h, ops.dequantize_rows(q, s), ops.linear_int8(q, s, q, s, x[0, :3])))
+    q, s, h = ops.add_rms_norm_int8(x)
+    assert h is x and h.requires_grad and not s.requires_grad
+
+
+# ------------------------------------------------------------------------------------------------ offsets beyond 32 bits
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(66000, 33000, 48), (66000, 40, 33000), (40, 66000, 33000), (3, 66000, 33000)])
+def test_products_whose_offsets_pass_32_bits(M, N, K):
+    """More than 2^31 results, activations' codes or weights' codes; rows and columns of both ends against 64 bits."""
+    def codes(rows, seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        kp = (K + 15) // 16 * 16
+        q = torch.randint(-127, 128, (rows, kp), generator=g, device="cuda", dtype=torch.int8)
+        return q[:, :K], torch.rand(rows, generator=g, device="cuda") * 0.01 + 1e-3
+
+    q, s = codes(M, 1)
+    w, ws = codes(N, 2)
+    y = ops.linear_int8(q, s, w, ws, None, "none", torch.bfloat16)
+    m = torch.unique(torch.cat([torch.arange(0, min(M, 40)), torch.arange(max(M - 40, 0), M)])).cuda()
+    n = torch.unique(torch.cat([torch.arange(0, min(N, 40)), torch.arange(max(N - 40, 0), N)])).cuda()
+    want = (q[m].double() @ w[n].double().t().contiguous()) * s[m].double()[:, None] * ws[n].double()
+    got = y[m][:, n].double()
+    assert torch.all((got - want).abs() <= (2.0 ** -8 + 2.0 ** -20) * want.abs() + 1e-30)
+
+
+@pytest.mark.gpu
+def test_rows_whose_offsets_pass_32_bits():
+    M, K = 33, (1 << 26) + 8
+    x = torch.zeros(M, K, dtype=torch.bfloat16, device="cuda")
+    x[:, 5], x[:, K - 1] = 2.0, -1.0
+    q, s = ops.quantize_rows(x)
+    assert torch.all(q[:, 5] == 127) and torch.all(q[:, K - 1] == -64) and torch.all(q.to(torch.int16).abs().sum(1, dtype=torch.int64) == 191)
+    back = ops.dequantize_rows(q, s, torch.bfloat16)
+    assert torch.all(back[:, 5] == 2.0) and torch.all(back[:, K - 2] == 0) and torch.all(back[:, K - 1] == (-64 * (torch.tensor(2.0) / 127)).bfloat16().item())
+    p, t, h = ops.add_rms_norm_int8(x, None, x)
+    assert torch.equal(h[-1], x[-1] * 2) and torch.equal(p[-1], q[-1])
