@@ -179,9 +179,9 @@ __device__ __forceinline__ void scale8(float (&y)[8], const void* weight, long l
     for (int i = 0; i < 8; ++i) y[i] *= (float)w.e[i];
 }
 
-// What bounds it is memory: quantising 8192 x 8192 bf16 takes 32.5 us (6.2 TB/s read and written), 2000 x 16384 fp32 25.7 us
-// (6.4), the norm with a residual of 4096 x 4096 bf16 22 us (5.3), of 16384 x 8192 175 us (5.4); a copy of 1 GiB runs at 5.2.
-// Rows of odd length (16384 x 1111 bf16, loads across cache lines) get 3.3 TB/s.
+// What bounds it is memory: quantising 8192 x 8192 bf16 takes 40 us (5.0 TB/s read and written), 2000 x 16384 fp32 33.8 us
+// (4.9), the norm with a residual of 4096 x 4096 bf16 27 us (4.4), of 16384 x 8192 175 us (5.4); a copy of 1 GiB runs at 5.2.
+// Rows of odd length (16384 x 1111 bf16, loads across cache lines) get 3.4 TB/s.  (Graph of calls on three sets of operands.)
 // A row stays in the registers of its G threads from the load to the codes: one read, one write, whatever is computed
 // between.  Thread t holds the 8-element chunks t, t + G, ... (V of them).
 template <typename T, int G, int V, bool NORM>
@@ -433,9 +433,9 @@ static int launch_rows(const QuantRowsArgs& a, long long threads, hipStream_t st
 template <typename T>
 static int launch_rows_of(const QuantRowsArgs& a, long long threads, hipStream_t stream) {
     // c: chunks of 8 a row needs.  Short rows share a wave, long ones take as few threads as hold them in 4 chunks each (8 from
-    // 8192 columns on); where the rows are fewer than the CUs, 1024 threads answer sooner than 256.  Measured: 65536 x 100 fp32
-    // 7.1 us, 18.5 with a wave
-    // a row; 1 x 16384 bf16 with a residual 5.0 us, 8.8 with 256 threads.
+    // 8192 columns on); where the rows are no more than the CUs, 1024 threads answer sooner than 256.  Measured (us): 65536 x 100
+    // fp32 8.9, 19.0 with a wave a row; bf16 with a residual, 1024 threads and 256: 1 x 16384 4.9 and 8.8, 1 x 5000 4.2 and 5.2,
+    // 256 x 16384 8.8 and 13.9, 256 x 5000 5.3 and 6.2.
     const long long c = a.ld_q >> 3;
     if (c <= 16) return launch_rows<T, 16, 1>(a, threads, stream);
     if (c <= 32) return launch_rows<T, 16, 2>(a, threads, stream);
@@ -470,7 +470,7 @@ D4PG_API int d4pg_quant_rows(const QuantRowsArgs* a, hipStream_t stream) { retur
 // codes -> floating rows
 // ---------------------------------------------------------------------------------------------------------------
 
-// 8192 x 8192 to bf16: 30.7 us (6.6 TB/s).
+// 8192 x 8192 to bf16: 38 us (5.3 TB/s); 30 us right after quantising, with the codes in the cache.
 template <typename T>
 __global__ __launch_bounds__(256) void dequant_rows_kernel(const DequantRowsArgs a) {
     const int tpr = 1 << a.tpr_log;
@@ -710,7 +710,7 @@ static int launch_linear_rows(const LinearInt8Args& a, long long threads, hipStr
 //
 // What bounds it at 8192^3 (tiles of 256): power first - the matrix instruction alone does 4.9 P/s on zeros, 3.5 on random
 // codes, 3.1 - 3.2 with its LDS reads - then how well the rest hides behind it.  Moves alone take 231 us.  Waves a SIMD
-// decide the rest: 1 (waves of 128 x 128) 560 us, matrix pipe 52 % busy; 2 (128 x 64) 476; 4 (64 x 64) 464 us = 2.37 P/s.
+// decide the rest: 1 (waves of 128 x 128) 560 us, matrix pipe 52 % busy; 2 (128 x 64) 476; 4 (64 x 64) 465 us = 2.36 P/s (pipe 70 %).
 enum { STEP_FULL = 0, STEP_DRAIN = 1, STEP_LAST = 2 };
 
 template <int MI, int NI, int WM, int WN, int KW, int S>
